@@ -83,6 +83,21 @@ class MoeFp8Layer(ctypes.Structure):
     ]
 
 
+class MlaPrefillArgs(ctypes.Structure):
+    _fields_ = [
+        ("q_nope", ctypes.c_void_p), ("ld_q_nope", ctypes.c_int64), ("hd_q_nope", ctypes.c_int64),
+        ("q_rope", ctypes.c_void_p), ("ld_q_rope", ctypes.c_int64), ("hd_q_rope", ctypes.c_int64),
+        ("k_nope", ctypes.c_void_p), ("ld_k_nope", ctypes.c_int64), ("hd_k_nope", ctypes.c_int64),
+        ("k_rope", ctypes.c_void_p), ("ld_k_rope", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("ld_v", ctypes.c_int64), ("hd_v", ctypes.c_int64),
+        ("cu_q", ctypes.c_void_p), ("cu_k", ctypes.c_void_p),
+        ("B", ctypes.c_int), ("Tq", ctypes.c_int), ("Tk", ctypes.c_int), ("max_q", ctypes.c_int), ("H", ctypes.c_int),
+        ("nope", ctypes.c_int), ("P", ctypes.c_int), ("vd", ctypes.c_int), ("causal", ctypes.c_int),
+        ("softmax_scale", ctypes.c_float), ("out", ctypes.c_void_p), ("ld_out", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
+    ]
+
+
 DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_F8E4M3 = 0, 1, 2, 3
 STREAM_LEGACY = 1  # cudaStreamLegacy: the legacy default stream as a stream handle
 
@@ -183,6 +198,14 @@ _PROTOS = [
     ("dsb_rmsnorm", ctypes.c_int, [_vp, _vp, _i64, _vp, _ci, _ci, _cf, _vp, _i64, _vp, _i64]),
     ("dsb_kv_norm_rope_append", ctypes.c_int,
      [_vp, _vp, _vp, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _cf, _cf, _vp, _vp]),
+    ("dsb_kv_norm_rope_append_fp8", ctypes.c_int,
+     [_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _ci, _cf, _cf, _vp, _vp, _i64,
+      _vp]),
+    ("dsb_mla_decode_fp8", ctypes.c_int,
+     [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _ci, _vp, _ci, _ci, _ci, _ci, _cf, _vp]),
+    ("dsb_mla_cache_read_fp8", ctypes.c_int,
+     [_vp, _vp, _vp, _i64, _vp, _ci, _vp, _ci, _i64, _ci, _ci, _vp, _i64, _vp, _i64]),
+    ("dsb_mla_prefill", ctypes.c_int, [_vp, ctypes.POINTER(MlaPrefillArgs)]),
     ("dsb_router_logits", ctypes.c_int, [_vp, _vp, _vp, _ci, _ci, _ci, _vp]),
     ("dsb_moe_route", ctypes.c_int, [_vp, _vp, _vp, _ci, _ci, _ci, _ci, _ci, _ci, _ci, _cf, _vp, _vp]),
     ("dsb_moe_permute", ctypes.c_int, [_vp, _vp, _ci, _ci, _ci, _vp, _vp, _vp, _vp, _vp, _vp]),
@@ -392,6 +415,46 @@ class Context:
         self._check(self._l.dsb_kv_norm_rope_append(
             self.h, _ptr(kv_a), _ptr(w_norm), _ptr(q), _ptr(positions), _ptr(block_table), block_table.shape[1], B,
             H, nope, R, P, float(eps), float(theta), _ptr(cache), _ptr(q_rope)))
+
+    # ---- 8-bit latent cache: cache uint8 [n_blocks, 64, R + 2P], scales fp32 [n_blocks, 64]
+    def kv_norm_rope_append_fp8(self, kv_a, w_norm, q, positions, block_table, H, nope, R, P, eps, theta, cache,
+                                scales, q_rope, seq_ids=None):
+        """dsb_kv_norm_rope_append_fp8: rows of kv_a [B, R+P] fp32 into the 8-bit cache, q_rope [B, H, P] rotated.
+        Row b belongs to sequence seq_ids[b] (None: b); a negative position marks padding."""
+        self._check(self._l.dsb_kv_norm_rope_append_fp8(
+            self.h, _ptr(kv_a), kv_a.stride(0), _ptr(w_norm), _ptr(q), q.stride(0), _ptr(positions), _ptr(seq_ids),
+            _ptr(block_table), block_table.shape[0], block_table.shape[1], kv_a.shape[0], H, nope, R, P, float(eps),
+            float(theta), _ptr(cache), _ptr(scales), cache.shape[0], _ptr(q_rope)))
+
+    def mla_decode_fp8(self, q_lat, q_rope, cache, scales, block_table, seq_lens, softmax_scale, out):
+        """dsb_mla_decode_fp8: q_lat [B, H, R], q_rope [B, H, P] bf16, seq_lens int32 [B] on the device -> out [B, H, R]."""
+        B, H, R = q_lat.shape
+        self._check(self._l.dsb_mla_decode_fp8(
+            self.h, _ptr(q_lat), _ptr(q_rope), _ptr(cache), _ptr(scales), cache.shape[0], _ptr(block_table),
+            block_table.shape[1], _ptr(seq_lens), B, H, R, q_rope.shape[2], float(softmax_scale), _ptr(out)))
+
+    def mla_cache_read_fp8(self, cache, scales, block_table, cu_seqlens, latent, k_rope):
+        """dsb_mla_cache_read_fp8: cached tokens as bf16 rows of latent [T, R] and k_rope [T, P]."""
+        T, R = latent.shape
+        self._check(self._l.dsb_mla_cache_read_fp8(
+            self.h, _ptr(cache), _ptr(scales), cache.shape[0], _ptr(block_table), block_table.shape[1],
+            _ptr(cu_seqlens), block_table.shape[0], T, R, k_rope.shape[1], _ptr(latent), latent.stride(0),
+            _ptr(k_rope), k_rope.stride(0)))
+
+    def mla_prefill(self, q_nope, q_rope, k_nope, k_rope, v, cu_q, cu_k, max_q, softmax_scale, out, causal=True,
+                    lse=None):
+        """dsb_mla_prefill on bf16 tensors [T, H, dim] (k_rope [T, P]) of any token and head pitch; out [Tq, H, vd]."""
+        Tq, H, nope = q_nope.shape
+        a = MlaPrefillArgs(
+            q_nope=_ptr(q_nope), ld_q_nope=q_nope.stride(0), hd_q_nope=q_nope.stride(1),
+            q_rope=_ptr(q_rope), ld_q_rope=q_rope.stride(0), hd_q_rope=q_rope.stride(1),
+            k_nope=_ptr(k_nope), ld_k_nope=k_nope.stride(0), hd_k_nope=k_nope.stride(1),
+            k_rope=_ptr(k_rope), ld_k_rope=k_rope.stride(0), v=_ptr(v), ld_v=v.stride(0), hd_v=v.stride(1),
+            cu_q=_ptr(cu_q), cu_k=_ptr(cu_k), B=cu_q.shape[0] - 1, Tq=Tq, Tk=k_nope.shape[0], max_q=int(max_q), H=H,
+            nope=nope, P=q_rope.shape[2], vd=v.shape[2], causal=int(causal), softmax_scale=float(softmax_scale),
+            out=_ptr(out), ld_out=out.stride(0), lse=_ptr(lse),
+        )
+        self._check(self._l.dsb_mla_prefill(self.h, ctypes.byref(a)))
 
     def router_logits(self, x, w_gate, logits):
         T, D = x.shape

@@ -180,6 +180,7 @@ int dsb_ctx_destroy(dsb_ctx* ctx) {
   if (ctx->step) cudaFree(ctx->step);
   if (ctx->perm) cudaFree(ctx->perm);
   if (ctx->moe) cudaFree(ctx->moe);
+  if (ctx->mla8) cudaFree(ctx->mla8);
   if (ctx->d_status) cudaFree(ctx->d_status);
   if (ctx->own_stream) cudaStreamDestroy(ctx->stream);
   delete ctx;

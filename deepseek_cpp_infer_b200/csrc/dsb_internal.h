@@ -32,6 +32,8 @@ struct dsb_ctx {
   size_t perm_bytes = 0;
   void* moe = nullptr;      // activations of dsb_moe_ffn_fp8
   size_t moe_bytes = 0;
+  void* mla8 = nullptr;     // split-KV partials of dsb_mla_decode_fp8 (allocated once, never regrown)
+  size_t mla8_bytes = 0;
   std::string last_error;
   dsb_stats stats{};
 };
@@ -140,6 +142,23 @@ int smem_attr_once(dsb_ctx* ctx, Kernel kernel, size_t bytes, std::atomic<bool> 
   }
   return DSB_OK;
 }
+
+// Makes `device` current for a scope and the caller's device current again
+// afterwards.
+struct DeviceScope {
+  int before = -1;
+  bool ok = false;
+  explicit DeviceScope(int device) {
+    if (cudaGetDevice(&before) != cudaSuccess) before = -1;
+    ok = before == device || cudaSetDevice(device) == cudaSuccess;
+    if (before == device) before = -1;
+  }
+  ~DeviceScope() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
 
 // Check a CUDA runtime call; on failure record it and return DSB_ECUDA.
 #define DSB_CUDA_TRY(ctx, call)                                                                     \

@@ -335,6 +335,117 @@ DSB_API int dsb_kv_norm_rope_append(dsb_ctx* ctx, const float* kv_a, const float
                                     const int32_t* positions, const int32_t* block_table, int max_blocks, int B, int H,
                                     int nope, int R, int P, float eps, float theta, void* cache, void* q_rope);
 
+/* ------------------------------------------------------ 8-bit latent cache
+ *
+ * A paged latent cache in 8 bits, 56% of the bf16 cache's bytes at R = 512,
+ * P = 64.  A cached token is
+ *   scale * [ latent (R values, e4m3) | rope key (P values, bf16) ]
+ * stored as one row of R + 2P bytes of `cache` (uint8 [n_blocks, 64, R + 2P],
+ * 16-byte aligned) and one fp32 of `scales` [n_blocks, 64].  The scale is the
+ * token's own power of two (a page-wide one would have to be requantised as
+ * tokens arrive; e4m3 carries an exponent, so a power of two costs range and
+ * no precision), and it covers the whole row: the rope part is the bf16 rope
+ * key divided by it, which is exact.  Every cached value is therefore exact
+ * in bf16.  The reference caches fp32 keys and values (MLACache,
+ * src/models/deepseek/mla.cpp:16-39) and has no 8-bit cache.
+ *
+ * Common to the calls below: (R, P) in {(512, 64), (128, 32)}, pages of 64
+ * tokens, device int32 block tables [n_seqs, max_blocks].  A page id outside
+ * [0, n_blocks), a position past the table or a length that the table cannot
+ * hold makes the kernel skip that access and sets the device status word:
+ * dsb_sync returns DSB_EINVAL.  All of them run on the context's device
+ * (whichever is current) and stream, and may be captured into a graph after a
+ * first call on the context outside of capture. */
+
+/* dsb_kv_norm_rope_append into the 8-bit cache, for B token rows of any
+ * sequences at any positions (a decode batch, or a prefill chunk):
+ *   c = rmsnorm(kv_a[b, :R]) * w_norm
+ *   scale = 2^ceil(log2(max|c| / 448)), exponent within [-64, 64]; 1 when c = 0
+ *   row = [ e4m3(c / scale) | bf16(rope(kv_a[b, R:R+P], pos)) / scale ]
+ *   q_rope[b, h] = bf16(rope(q[b, h, nope:nope+P], pos))
+ * Row b belongs to sequence seq_ids[b] (device int32, NULL: sequence b) at
+ * positions[b]; a row with a negative position is padding: neither the cache
+ * nor its q_rope is written.  Norm and angles are computed in 64 bits, so
+ * codes and far positions do not depend on summation order.  The interleaved
+ * pair convention of dsb_kv_norm_rope_append.  No two rows may name the same
+ * position of a sequence.
+ * kv_a fp32 [B, R+P] (row pitch ld_kv, a multiple of 4), q bf16 [B, H*(nope+P)]
+ * (row pitch ldq), q_rope bf16 [B, H, P]; kv_a, w_norm, q, q_rope 16-byte
+ * aligned; nope and ldq multiples of 8. */
+DSB_API int dsb_kv_norm_rope_append_fp8(dsb_ctx* ctx, const float* kv_a, int64_t ld_kv, const float* w_norm,
+                                        const void* q, int64_t ldq, const int32_t* positions, const int32_t* seq_ids,
+                                        const int32_t* block_table, int n_seqs, int max_blocks, int B, int H, int nope,
+                                        int R, int P, float eps, float theta, void* cache, float* scales,
+                                        int64_t n_blocks, void* q_rope);
+
+/* dsb_mla_decode over the 8-bit cache: one query token per sequence,
+ *   out_lat[b, h] = sum_j softmax_j(softmax_scale * [q_lat | q_rope] . row_j) * latent_j
+ * over the seq_lens[b] cached tokens of sequence b (a length of 0 gives a zero
+ * row).  seq_lens is a DEVICE int32 [B]: the kernel splits the work itself, so
+ * a captured call may be replayed with other lengths.  Cache rows past a
+ * length are not used, whatever they hold.  Scratch comes from the context
+ * (39 MB, allocated by the first call): calls of one context must not overlap
+ * on the GPU.  H <= 128; q_lat, q_rope, out_lat bf16 as in dsb_mla_decode,
+ * 16-byte aligned; n_blocks <= 2^25 - 1. */
+DSB_API int dsb_mla_decode_fp8(dsb_ctx* ctx, const void* q_lat, const void* q_rope, const void* cache,
+                               const float* scales, int64_t n_blocks, const int32_t* block_table, int max_blocks,
+                               const int32_t* seq_lens, int B, int H, int R, int P, float softmax_scale,
+                               void* out_lat);
+
+/* Read cached tokens back as bf16 rows, for the re-expansion of a history
+ * (k_nope | v = kv_b_proj . latent) in front of a dsb_mla_prefill chunk.
+ * Sequence b's first cu_seqlens[b+1] - cu_seqlens[b] tokens go to rows
+ * cu_seqlens[b] .. of latent [T, R] (row pitch ld_lat) and k_rope [T, P] (row
+ * pitch ld_rope); either may be NULL.  cu_seqlens device int32 [B + 1],
+ * ascending from 0; rows at or past cu_seqlens[B] (T is the buffers' row
+ * count) are left as they were.  Exact.  Outputs 16-byte aligned, pitches
+ * multiples of 8. */
+DSB_API int dsb_mla_cache_read_fp8(dsb_ctx* ctx, const void* cache, const float* scales, int64_t n_blocks,
+                                   const int32_t* block_table, int max_blocks, const int32_t* cu_seqlens, int B,
+                                   int64_t T, int R, int P, void* latent, int64_t ld_lat, void* k_rope,
+                                   int64_t ld_rope);
+
+/* Prompt attention in expanded form: the per-head attention of
+ * mla_decode_step (src/models/deepseek/mla.cpp:86-116) for whole chunks of
+ * query rows of several sequences,
+ *   s_ij = ([q_nope_ih | q_rope_ih] . [k_nope_jh | k_rope_j]) * softmax_scale
+ *   out_ih = sum_j softmax_j(s_ij) v_jh,   lse_ih = ln sum_j exp(s_ij)
+ * with the rope key shared by the heads.  Sequence b has query rows
+ * cu_q[b] .. cu_q[b+1] and key rows cu_k[b] .. cu_k[b+1] (device int32 [B + 1],
+ * ascending from 0, at most Tq and Tk); with `causal`, its i-th query sees
+ * its keys j <= i + len_k - len_q (the last query sees every key).  A query
+ * that sees none gets a zero row and lse = -inf.  Query rows at or past
+ * cu_q[B] are left as they were.  max_q bounds any sequence's query rows: it
+ * sizes the grid, and rows beyond it set the status word (dsb_sync returns
+ * DSB_EINVAL) and are left as they were.
+ * All tensors bf16 with a token pitch ld_* and, where there are heads, a head
+ * pitch hd_* in elements, multiples of 8 (so k_nope and v may be the two
+ * halves of one kv_b projection, q_nope the front of each head of q);
+ * pointers 16-byte aligned.  out [Tq, ld_out], head h at column h * vd; lse
+ * fp32 [Tq, H] or NULL.  Supported (nope, P, vd): (128, 64, 128), (64, 32, 64). */
+typedef struct dsb_mla_prefill_args {
+  const void* q_nope;
+  int64_t ld_q_nope, hd_q_nope;
+  const void* q_rope;
+  int64_t ld_q_rope, hd_q_rope;
+  const void* k_nope;
+  int64_t ld_k_nope, hd_k_nope;
+  const void* k_rope;
+  int64_t ld_k_rope;
+  const void* v;
+  int64_t ld_v, hd_v;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int B, Tq, Tk, max_q, H, nope, P, vd;
+  int causal;
+  float softmax_scale;
+  void* out;
+  int64_t ld_out;
+  float* lse;
+} dsb_mla_prefill_args;
+
+DSB_API int dsb_mla_prefill(dsb_ctx* ctx, const dsb_mla_prefill_args* args);
+
 /* fp32 router logits [T, E] = x [T, D] . W_gate [E, D]^T (ops.cpp:115-117). */
 DSB_API int dsb_router_logits(dsb_ctx* ctx, const float* x, const float* w_gate, int T, int D, int E, float* logits);
 
