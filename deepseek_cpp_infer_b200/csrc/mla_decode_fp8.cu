@@ -1,12 +1,46 @@
-// Absorbed MLA decode attention over the 8-bit paged latent cache.
+// Absorbed MLA decode attention over the 8-bit paged latent cache, sm_100a.
 //
-//   s_j = softmax_scale * scale_j * (q_lat . c8_j + q_rope . kr_j)
-//   out = sum_j softmax(s)_j * scale_j * c8_j
+//   s_j = softmax_scale * sigma_j * (q_lat . c8_j + q_rope . kr_j)
+//   out = sum_j softmax(s)_j * sigma_j * c8_j
+// (c8_j the token's e4m3 latents, kr_j its bf16 rope part, sigma_j its scale).
+//
+// The cached bytes are tensor-core operands as they are stored; nothing is
+// converted.  Tokens are the MMA's M: a tile is 128 tokens (two pages), and
+//   S^T [128 tokens x heads] = C8 . Q^T  (+ KR . Qr^T, kind::f16)
+//   O^T [R x heads] per tile  = C8^T . P (the same bytes, MN-major)
+// so that few heads cost few columns and the tile is read once for both
+// products.
+//
+// Precision.  An e4m3 value has 4 significant bits, a bf16 query 8: q / a (a
+// a power of two per head) is split into hi = e4m3(q / a) and lo = e4m3(q / a
+// - hi), exact down to 2^-18 of the head's largest value.  hi and lo are
+// separate columns of one MMA (N = 2 heads), summed in fp32.  Probabilities
+// are split the same way (8 significant bits, like bf16), in units of their
+// own tile's maximum: each tile's O^T is a fresh accumulator that is added to
+// fp32 registers with the tile's weight, so that thousands of small
+// probabilities behind one large one (an attention sink) keep their digits.
+// The token's scale joins its probability: with u = s log2(e) + log2(sigma),
+// p' = 2^(u - max u) carries sigma, and the softmax sum takes p' / sigma.
+//
+// Work.  Sequences' tiles in order, cut into one even run per SM (per head
+// group of up to 64 heads; both groups of 128 heads walk the same tiles at
+// the same time and share them through L2).  The lengths are read on the
+// device.  A run's first and last sequences may be shared with its neighbours:
+// such segments go to fp32 partials that combine_kernel merges.
+//
+// Roles (10 warps): 8 softmax / accumulate warps, two warpgroups with half of
+// the heads each (thread = token for S^T, thread = latent column for O^T), a
+// TMA warp and an MMA warp.  Shared memory is a ring of 128-token x 128-byte
+// slabs (R / 128 of latents and one of rope keys per tile): a slab serves QK
+// and, as soon as its block of O^T is done, is free again, so that at 64 heads
+// (72 KB of query digits) 8 slabs suffice to run the next tile's QK ahead of
+// this tile's PV.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "dsb_internal.h"
@@ -16,82 +50,812 @@
 namespace dsb {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kTileTok = 128;       // tokens per tile: MMA M
+constexpr int kSmWarps = 8;         // softmax / accumulate warps
+constexpr int kThreads = (kSmWarps + 2) * 32;
+constexpr int kMaxHeadsPerCta = 64;
+constexpr int kMaxSeqs = 65536;     // prefix array in the scratch
+constexpr int kScaleStages = 4;
 
-// One CTA per (sequence, head); a warp takes every 8th token with its own
-// running maximum, sum and R / 32 output columns per lane; the warps' states
-// are merged in shared memory.
-template <int R, int P>
-__global__ void __launch_bounds__(kWarps * 32)
-    decode_fp8_kernel(const __nv_bfloat16* __restrict__ q_lat, const __nv_bfloat16* __restrict__ q_rope,
-                      const uint8_t* __restrict__ cache, const float* __restrict__ scales, int64_t n_blocks,
-                      const int32_t* __restrict__ block_table, int max_blocks, const int32_t* __restrict__ seq_lens,
-                      int H, float scale_log2, __nv_bfloat16* __restrict__ out, int* __restrict__ status) {
-  constexpr int NR = R / 32, NP = P / 32;
+template <int R, int P, int HB>
+struct Shape {
+  static constexpr int NL = R / 128;                 // latent slabs per tile
+  static constexpr int NSLAB = NL + 1;               // + rope
+  static constexpr int HW = HB / 2;                  // heads per warpgroup
+  static constexpr int SLAB = kTileTok * 128;        // bytes
+  static constexpr int NS = HB == 16 ? 12 : HB == 32 || NL == 1 ? 10 : 8;  // ring slots: what fits
+  // slabs of tile n + 1's QK issued before tile n's PV: all when two tiles
+  // fit, else as many as the ring can hold beside tile n's latents
+  static constexpr int LA = NS >= 2 * NSLAB ? NSLAB : NS - NL;
+  static_assert(LA >= 1 && LA <= NSLAB, "ring");
+  static constexpr int Q8_BYTES = 2 * HB * R;        // [slab][hi heads | lo heads][128 B], SW128
+  static constexpr int QR_BYTES = HB * P * 2;        // [head][P bf16], SW128 (P = 64) or SW64
+  static constexpr int P_BYTES = HB * kTileTok;      // one digit of the probabilities
+  static constexpr int OFF_RING = 0;
+  static constexpr int OFF_Q8 = OFF_RING + NS * SLAB;
+  static constexpr int OFF_QR = OFF_Q8 + Q8_BYTES;
+  static constexpr int OFF_P = OFF_QR + QR_BYTES;
+  static constexpr int OFF_SC = OFF_P + 2 * P_BYTES;                     // [stages][128] token scales
+  static constexpr int OFF_RED = OFF_SC + kScaleStages * kTileTok * 4;   // [2 parity][2 wg][4 warps][HW] maxima
+  static constexpr int OFF_LRED = OFF_RED + 2 * 2 * 4 * HW * 4;          // [2 wg][4 warps][HW] sums
+  static constexpr int OFF_AB = OFF_LRED + 2 * 4 * HW * 4;               // per warp [2][HW]: old and tile weights
+  static constexpr int OFF_MT = OFF_AB + kSmWarps * 2 * HW * 4;          // per warp [HW]: tile maxima (or 1 / sums)
+  static constexpr int OFF_FH = OFF_MT + kSmWarps * HW * 4;              // [HB] a_h * scale * log2(e)
+  static constexpr int NBAR = 2 * NS + 2 + NL + 6 + 2 * kScaleStages;
+  static constexpr int OFF_BAR = (OFF_FH + HB * 4 + 7) / 8 * 8;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;                    // tmem base, abort flags, scan, start
+  static constexpr int SMEM_BYTES = OFF_MISC + 128 + 1024;               // + alignment slack
+  static_assert(SMEM_BYTES <= 232448, "shared memory");
+  static_assert(OFF_Q8 % 1024 == 0 && OFF_QR % 1024 == 0 && OFF_P % 128 == 0 && OFF_SC % 16 == 0, "alignment");
+  // TMEM columns: S^T two buffers of [hi | lo], then O^T, one block of HB columns per latent slab
+  static constexpr uint32_t T_S = 0, T_O = 4 * HB;
+  static constexpr int USED = 4 * HB + NL * HB;
+  static constexpr uint32_t T_COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+  static_assert(USED <= 512, "TMEM");
+};
+
+__device__ __forceinline__ float redux_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// Two floats as e4m3 digits: hi = e4m3(v), lo = e4m3(v - hi), through fp16 (11
+// significant bits; the difference is exact).
+__device__ __forceinline__ void split_digits(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const uint32_t v = pack_half2(a, b);
+  uint16_t h, l;
+  uint32_t hf, d;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(v));
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hf) : "h"(h));
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(hf));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l) : "r"(d));
+  hi = h;
+  lo = l;
+}
+
+// 1D bulk copy global -> shared, completing on `bar` (addresses and size multiples of 16).
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
+  uint32_t r[N];
+  if constexpr (N == 32) tmem_ld32(taddr, r);
+  else if constexpr (N == 16) tmem_ld16(taddr, r);
+  else tmem_ld8(taddr, r);
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ bool bad_len(int len, int max_blocks) {
+  return len < 0 || len > (int64_t)max_blocks * kPageTok;
+}
+
+__device__ __forceinline__ int tiles_of(int len, int max_blocks) {
+  return bad_len(len, max_blocks) ? 0 : (int)(((int64_t)len + kTileTok - 1) / kTileTok);
+}
+
+// A run of tiles through the sequences; every role walks its own copy.
+struct Walk {
+  const int32_t* lens;
+  int B, max_blocks;
+  int b, tile, ntile, len;
+  __device__ void start(const int32_t* l, int B_, int mb, int b_, int tile_) {
+    lens = l;
+    B = B_;
+    max_blocks = mb;
+    b = b_;
+    tile = tile_;
+    len = lens[b];
+    ntile = tiles_of(len, max_blocks);
+  }
+  __device__ void next() {  // only called while tiles are left
+    if (++tile < ntile) return;
+    tile = 0;
+    do {
+      ++b;
+      len = b < B ? lens[b] : 1;
+      ntile = tiles_of(len, max_blocks);
+    } while (ntile == 0);
+  }
+  __device__ int valid() const { return min(kTileTok, len - tile * kTileTok); }  // tokens of this tile
+};
+
+// First tile of run i of n over T tiles.
+__device__ __forceinline__ int64_t run_start(int64_t i, int64_t T, int n) { return i * T / n; }
+// The run that holds tile t.
+__device__ __forceinline__ int run_of(int64_t t, int64_t T, int n) { return (int)(((t + 1) * n - 1) / T); }
+
+template <int R, int P, int HB>
+__global__ void __launch_bounds__(kThreads, 1)
+    decode_fp8_kernel(const __grid_constant__ CUtensorMap map_lat, const __grid_constant__ CUtensorMap map_rope,
+                      const __nv_bfloat16* __restrict__ q_lat, const __nv_bfloat16* __restrict__ q_rope,
+                      const float* __restrict__ scales, int64_t n_blocks, const int32_t* __restrict__ block_table,
+                      int max_blocks, const int32_t* __restrict__ seq_lens, int B, int H, int runs, float scale_log2,
+                      __nv_bfloat16* __restrict__ out, float* __restrict__ ws_o, float2* __restrict__ ws_ml,
+                      int32_t* __restrict__ prefix, int* __restrict__ status) {
+  using S = Shape<R, P, HB>;
+  constexpr int NL = S::NL, NS = S::NS, HW = S::HW, NSLAB = S::NSLAB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
+  uint64_t* full = bars;                     // [NS] slab landed
+  uint64_t* empty = full + NS;               // [NS] slab's last MMA done
+  uint64_t* s_full = empty + NS;             // [2] scores of a tile ready
+  uint64_t* o_full = s_full + 2;             // [NL] a block of the tile's O^T ready
+  uint64_t* p_full = o_full + NL;            // probabilities of a tile written
+  uint64_t* o_free = p_full + 1;             // O^T of a tile taken into registers
+  uint64_t* q_ready = o_free + 1;            // query digits of a segment written
+  uint64_t* wg_bar = q_ready + 1;            // [2] rendezvous of a warpgroup
+  uint64_t* sc_full = wg_bar + 2;            // [stages] token scales landed
+  uint64_t* sc_empty = sc_full + kScaleStages;
+  uint64_t* drain = sc_empty + kScaleStages;  // every MMA issued is done
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + S::OFF_MISC);
+  volatile int* abort = reinterpret_cast<volatile int*>(misc + 1);
+  volatile int* no_abort = reinterpret_cast<volatile int*>(misc + 2);  // never raised: for drain waits
+  int* start = reinterpret_cast<int*>(misc + 3);                       // sequence and tile of the run's start
+  int* scan = reinterpret_cast<int*>(misc + 8);                        // [10] warp totals
+
+  const int warp = (int)warp_id(), lane = (int)lane_id();
+  const int hg = blockIdx.x / runs, run = blockIdx.x % runs;  // head group and run
+  constexpr int kTmaWarp = kSmWarps, kMmaWarp = kSmWarps + 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&wg_bar[i], kSmWarps / 2);
+    }
+    for (int i = 0; i < NL; ++i) mbar_init(&o_full[i], 1);
+    mbar_init(p_full, kSmWarps);
+    mbar_init(o_free, kSmWarps);
+    mbar_init(q_ready, kSmWarps);
+    mbar_init(drain, 1);
+    for (int i = 0; i < kScaleStages; ++i) {
+      mbar_init(&sc_full[i], 1);
+      mbar_init(&sc_empty[i], kSmWarps);
+    }
+    *abort = 0;
+    *no_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(misc, S::T_COLS);
+    tmem_relinquish();
+  }
+  if (warp == kTmaWarp && lane == 0) {
+    tma_prefetch_desc(&map_lat);
+    tma_prefetch_desc(&map_rope);
+  }
   pdl_wait();
   pdl_launch_dependents();
-  const int b = blockIdx.x, h = blockIdx.y;
-  const int lane = (int)lane_id(), warp = (int)warp_id();
-  int len = seq_lens[b];
-  if (len < 0 || len > (int64_t)max_blocks * kPageTok) {
-    if (threadIdx.x == 0) atomicCAS(status, 0, kStatusBadInput);
-    len = 0;
-  }
-  float q[NR + NP], o[NR];
-#pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    q[i] = __bfloat162float(q_lat[((int64_t)b * H + h) * R + lane * NR + i]);
-    o[i] = 0.0f;
-  }
-#pragma unroll
-  for (int i = 0; i < NP; ++i) q[NR + i] = __bfloat162float(q_rope[((int64_t)b * H + h) * P + lane * NP + i]);
-  float m = -INFINITY, l = 0.0f;
-  for (int j = warp; j < len; j += kWarps) {
-    const int64_t page = block_table[(int64_t)b * max_blocks + j / kPageTok];
-    if (page < 0 || page >= n_blocks) {
-      if (lane == 0) atomicCAS(status, 0, kStatusBadInput);
-      continue;
+
+  // Tiles before each thread's share of the sequences, and this CTA's run.
+  int64_t run0, count;
+  {
+    const int per = (B + kThreads - 1) / kThreads;
+    const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int len = seq_lens[b];
+      if (blockIdx.x == 0 && bad_len(len, max_blocks)) atomicCAS(status, 0, kStatusBadInput);
+      mine += tiles_of(len, max_blocks);
     }
-    const uint8_t* row = cache + (page * kPageTok + j % kPageTok) * (R + 2 * P);
-    const float sc = scales[page * kPageTok + j % kPageTok];
-    float k[NR];
-    float dot = 0.0f;
+    int inc = mine;
 #pragma unroll
-    for (int i = 0; i < NR; i += 2) {
-      const float2 f = unpack_half2(e4m3x2_to_half2(*reinterpret_cast<const uint16_t*>(row + lane * NR + i)));
-      k[i] = f.x;
-      k[i + 1] = f.y;
-      dot += q[i] * f.x + q[i + 1] * f.y;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
     }
+    if (lane == 31) scan[warp] = inc;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    int before = inc - mine, T = 0;
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
-      dot += q[NR + i] * __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row + R)[lane * NP + i]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    const float s = dot * sc * scale_log2;
-    const float mn = fmaxf(m, s);
-    const float a = exp2f(m - mn), p = exp2f(s - mn);
-    m = mn;
-    l = l * a + p;
-#pragma unroll
-    for (int i = 0; i < NR; ++i) o[i] = o[i] * a + p * sc * k[i];
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += scan[w];
+      T += scan[w];
+    }
+    run0 = run_start(run, T, runs);
+    count = run_start(run + 1, T, runs) - run0;
+    if (count > 0 && run0 >= before && run0 < before + mine) {
+      int t = before, b = b0;
+      for (;; ++b) {
+        const int n = tiles_of(seq_lens[b], max_blocks);
+        if (run0 < t + n) break;
+        t += n;
+      }
+      start[0] = b;
+      start[1] = (int)run0 - t;
+    }
+    if (blockIdx.x == 0) {  // for combine_kernel
+      int t = before;
+      for (int b = b0; b < b1; ++b) {
+        prefix[b] = t;
+        t += tiles_of(seq_lens[b], max_blocks);
+      }
+      if (threadIdx.x == 0) prefix[B] = T;
+    }
+    __syncthreads();
   }
-  __shared__ float sm[kWarps], sl[kWarps], so[kWarps][R];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
+  const uint32_t tmem = misc[0];
+  const uint32_t smem_base = smem_u32(smem);
+  Walk w;
+  if (count > 0) w.start(seq_lens, B, max_blocks, start[0], start[1]);
+
+  if (warp == kTmaWarp) {
+    // ------------------------------------------------------------ TMA producer
+    // Slab order per tile: rope, latents 0 .. NL - 1 (the rope slab is free
+    // again after QK, so its slot goes to the next tile's slab first).
+    if (lane == 0 && count > 0) {
+      const uint64_t policy = l2_policy_evict_first();
+      int it = 0;  // slabs issued
+      int nsc = 0; // scale stages issued
+      bool ok = true;
+      for (int64_t n = 0; ok && n < count; ++n) {
+        if (n > 0) w.next();
+        const int np = w.valid() > kPageTok ? 2 : 1;
+        int page[2] = {0, 0};
+        for (int p = 0; p < np; ++p) {
+          page[p] = block_table[(int64_t)w.b * max_blocks + w.tile * 2 + p];
+          if (page[p] < 0 || page[p] >= n_blocks) {  // read some page instead, and report it
+            page[p] = 0;
+            atomicCAS(status, 0, kStatusBadInput);
+          }
+        }
+        const int sc = (int)(n % kScaleStages);
+        if (n >= kScaleStages && !mbar_wait(&sc_empty[sc], (uint32_t)(n / kScaleStages - 1) & 1u, abort)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&sc_full[sc], np * kPageTok * 4);
+        for (int p = 0; p < np; ++p)
+          bulk_load(smem + S::OFF_SC + (sc * kTileTok + p * kPageTok) * 4, scales + (int64_t)page[p] * kPageTok,
+                    kPageTok * 4, &sc_full[sc]);
+        ++nsc;
+        for (int k = 0; k < NSLAB; ++k, ++it) {
+          const int slot = it % NS;
+          if (it >= NS && !mbar_wait(&empty[slot], (uint32_t)(it / NS - 1) & 1u, abort)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = smem + S::OFF_RING + slot * S::SLAB;
+          const int row = k == 0 ? P * 2 : 128;  // bytes of a slab's row
+          mbar_arrive_expect_tx(&full[slot], np * kPageTok * row);
+          for (int p = 0; p < np; ++p) {
+            if (k == 0) tma_load_2d(dst + p * kPageTok * row, &map_rope, &full[slot], R, page[p] * kPageTok, policy);
+            else tma_load_2d(dst + p * kPageTok * row, &map_lat, &full[slot], (k - 1) * 128, page[p] * kPageTok, policy);
+          }
+        }
+      }
+      if (!ok) raise_abort(abort, status, kStatusTimeout);
+      // every copy must land before shared memory is released, also when a
+      // consumer has given up
+      for (int i = max(0, it - NS); i < it; ++i) mbar_wait(&full[i % NS], (uint32_t)(i / NS) & 1u, no_abort);
+      for (int i = max(0, nsc - kScaleStages); i < nsc; ++i)
+        mbar_wait(&sc_full[i % kScaleStages], (uint32_t)(i / kScaleStages) & 1u, no_abort);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------- MMA issuer
+    if (lane == 0 && count > 0) {
+      constexpr uint32_t kMN = (1u << 15) | (1u << 16);  // A and B MN-major
+      constexpr uint32_t ID_QK = idesc_e4m3_f32(128, 2 * HB), ID_QR = idesc_bf16_f32(128, HB, 0, 0);
+      constexpr uint32_t ID_PV = idesc_e4m3_f32(128, HB) | kMN;
+      // operands' descriptors but for the slab's address
+      const uint64_t d_q8 = smem_desc(smem_base + S::OFF_Q8, 16, 1024, kSwizzle128B);
+      const uint64_t d_qr = P == 64 ? smem_desc(smem_base + S::OFF_QR, 16, 1024, kSwizzle128B)
+                                    : smem_desc(smem_base + S::OFF_QR, 16, 512, kSwizzle64B);
+      // P digits, no swizzle: 16 heads x 8 tokens per 128-byte core matrix,
+      // token groups 128 bytes apart, head groups 2048
+      const uint64_t d_p = smem_desc(smem_base + S::OFF_P, 128, kTileTok * 16, kSwizzleNone);
+      const uint64_t d_slab = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
+      const uint64_t d_rope = P == 64 ? d_slab : smem_desc(smem_base + S::OFF_RING, 16, 512, kSwizzle64B);
+      auto slot_of = [&](int64_t n, int k) { return (int)((n * NSLAB + k) % NS); };
+      auto parity_of = [&](int64_t n, int k) { return (uint32_t)((n * NSLAB + k) / NS) & 1u; };
+      bool ok = true;
+      // step 0: latents 0; step 1: rope; steps 2 ..: latents 1 ..
+      auto qk_step = [&](int64_t n, int step) {
+        const int k = step == 0 ? 1 : step == 1 ? 0 : step;  // slab of the tile, in load order
+        const int slot = slot_of(n, k);
+        if (!mbar_wait(&full[slot], parity_of(n, k), abort)) return false;
+        tc_fence_after();
+        const uint32_t d = tmem + S::T_S + (uint32_t)(n & 1) * 2 * HB;
+        const uint64_t off = (uint64_t)(slot * S::SLAB) >> 4;
+        if (k == 0) {
 #pragma unroll
-  for (int i = 0; i < NR; ++i) so[warp][lane * NR + i] = o[i];
+          for (int ks = 0; ks < P / 16; ++ks) mma_bf16_ss(d, d_rope + off + ks * 2, d_qr + ks * 2, ID_QR, 1u);
+          tc_commit(&empty[slot]);
+        } else {
+          const uint64_t qoff = (uint64_t)((k - 1) * 2 * HB * 128) >> 4;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            mma_f8_ss(d, d_slab + off + ks * 2, d_q8 + qoff + ks * 2, ID_QK, k > 1 || ks > 0 ? 1u : 0u);
+        }
+        return true;
+      };
+      int seg = 0;  // segments begun
+      ok = mbar_wait(q_ready, 0, abort);
+      ++seg;
+      for (int s = 0; ok && s < NSLAB; ++s) ok = qk_step(0, s);
+      if (ok) tc_commit(&s_full[0]);
+      for (int64_t n = 0; ok && n < count; ++n) {
+        const bool more = n + 1 < count;
+        bool fresh = false;  // tile n + 1 begins a sequence
+        if (more) {
+          w.next();
+          fresh = w.tile == 0;
+        }
+        int s = 0;
+        if (more && !fresh)
+          for (; ok && s < S::LA; ++s) ok = qk_step(n + 1, s);
+        if (ok && more && !fresh && S::LA == NSLAB) tc_commit(&s_full[(n + 1) & 1]);
+        if (!ok || !mbar_wait(p_full, (uint32_t)n & 1u, abort)) { ok = false; break; }
+        if (n > 0 && !mbar_wait(o_free, (uint32_t)(n - 1) & 1u, abort)) { ok = false; break; }
+        tc_fence_after();
+        for (int g = 0; g < NL; ++g) {
+          const int slot = slot_of(n, 1 + g);
+          const uint64_t a = d_slab + ((uint64_t)(slot * S::SLAB) >> 4);
+          const uint32_t d = tmem + S::T_O + g * HB;
+#pragma unroll
+          for (int ks = 0; ks < kTileTok / 32; ++ks) {
+            mma_f8_ss(d, a + ks * (4096 >> 4), d_p + ks * (512 >> 4), ID_PV, ks > 0 ? 1u : 0u);
+            mma_f8_ss(d, a + ks * (4096 >> 4), d_p + (S::P_BYTES >> 4) + ks * (512 >> 4), ID_PV, 1u);
+          }
+          tc_commit(&o_full[g]);
+          tc_commit(&empty[slot]);
+        }
+        if (more && (fresh || S::LA < NSLAB)) {
+          if (fresh) {
+            if (!mbar_wait(q_ready, (uint32_t)seg & 1u, abort)) { ok = false; break; }
+            ++seg;
+          }
+          for (; ok && s < NSLAB; ++s) ok = qk_step(n + 1, s);
+          if (ok) tc_commit(&s_full[(n + 1) & 1]);
+        }
+      }
+      if (!ok) raise_abort(abort, status, kStatusTimeout);
+      // every issued MMA must finish before TMEM and shared memory are released
+      tc_commit(drain);
+      mbar_wait(drain, 0, no_abort);
+    }
+  } else if (count > 0) {
+    // ------------------------------------------- softmax / accumulate warps
+    const int wg = warp >> 2, quarter = warp & 3;
+    const int j = quarter * 32 + lane;  // token of the tile; row of an O^T block
+    const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
+    float* red = reinterpret_cast<float*>(smem + S::OFF_RED);
+    float* lred = reinterpret_cast<float*>(smem + S::OFF_LRED);
+    float* ab = reinterpret_cast<float*>(smem + S::OFF_AB) + warp * 2 * HW;
+    float* mt = reinterpret_cast<float*>(smem + S::OFF_MT) + warp * HW;
+    float* fh = reinterpret_cast<float*>(smem + S::OFF_FH);
+    const int h0 = hg * HB;  // first head of the group
+
+    // Query digits of sequence b: a warp per head, 16 (4) latents a lane.  A
+    // warpgroup loads its own heads: its warps have all read the old factors
+    // (fh) when one of them is past the tile's rendezvous.
+    auto load_q = [&](int b) {
+      constexpr int CPL = R / 32;  // latents per lane
+#pragma unroll 1
+      for (int h = wg * HW + quarter; h < (wg + 1) * HW; h += 4) {
+        const bool live = h0 + h < H;
+        const int64_t row = (int64_t)b * H + h0 + h;
+        uint32_t x[CPL / 2];
+        uint4 r = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < CPL / 2; ++i) x[i] = 0;
+        if (live) {
+          if constexpr (CPL == 16) {
+            const uint4* src = reinterpret_cast<const uint4*>(q_lat + row * R + lane * 16);
+            const uint4 u = src[0], v = src[1];
+            x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(q_lat + row * R + lane * 4);
+            x[0] = u.x, x[1] = u.y;
+          }
+          if (lane < P / 8) r = *reinterpret_cast<const uint4*>(q_rope + row * P + lane * 8);
+        }
+        const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
+        float am = 0.0f, rm = 0.0f;
+#pragma unroll
+        for (int i = 0; i < CPL / 2; ++i) am = fmaxf(am, fmaxf(fabsf(bf16lo_to_f32(x[i])), fabsf(bf16hi_to_f32(x[i]))));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rm = fmaxf(rm, fmaxf(fabsf(bf16lo_to_f32(rr[i])), fabsf(bf16hi_to_f32(rr[i]))));
+        // the latents' scale; a rope part over 64 times larger sets it
+        // instead (it is divided by the same factor, in bf16, exactly)
+        const float top = redux_max(fmaxf(am, rm * 0.015625f));
+        const int e = min(100, max(-100, top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 7 : 0));
+        const float inv = exp2i(-e);
+        uint32_t hi[CPL / 4], lo[CPL / 4];
+#pragma unroll
+        for (int i = 0; i < CPL / 4; ++i) {
+          uint32_t a, b2, c, d;
+          split_digits(bf16lo_to_f32(x[2 * i]) * inv, bf16hi_to_f32(x[2 * i]) * inv, a, b2);
+          split_digits(bf16lo_to_f32(x[2 * i + 1]) * inv, bf16hi_to_f32(x[2 * i + 1]) * inv, c, d);
+          hi[i] = a | (c << 16);
+          lo[i] = b2 | (d << 16);
+        }
+        // row h (hi) and HB + h (lo) of each 128-column slab, 16-byte chunk c
+        // of a row at c ^ (row & 7)
+        const int col = lane * CPL, slab = col / 128, chunk = (col % 128) / 16, in = col % 16;
+        uint8_t* q8 = smem + S::OFF_Q8 + slab * 2 * HB * 128 + ((chunk ^ (h & 7)) * 16) + in;
+        if constexpr (CPL == 16) {
+          *reinterpret_cast<uint4*>(q8 + h * 128) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(q8 + (HB + h) * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        } else {
+          *reinterpret_cast<uint32_t*>(q8 + h * 128) = hi[0];
+          *reinterpret_cast<uint32_t*>(q8 + (HB + h) * 128) = lo[0];
+        }
+        if (lane < P / 8) {
+          uint32_t o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(bf16lo_to_f32(rr[i]) * inv, bf16hi_to_f32(rr[i]) * inv);
+          const int c = P == 64 ? (lane ^ (h & 7)) : (lane ^ ((h >> 1) & 3));
+          *reinterpret_cast<uint4*>(smem + S::OFF_QR + h * (P * 2) + c * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        if (lane == 0) fh[h] = exp2i(e) * scale_log2;
+      }
+      fence_proxy_async_shared();
+      warp_arrive(q_ready);
+    };
+
+    float acc[NL][HW];
+    float m_run = -INFINITY, l_run = 0.0f;  // of head lane % HW, the sum over this warp's tokens
+#pragma unroll
+    for (int g = 0; g < NL; ++g)
+#pragma unroll
+      for (int h = 0; h < HW; ++h) acc[g][h] = 0.0f;
+    int meet = 0;  // phase of wg_bar
+    bool ok = true;
+    bool shared_front = w.tile != 0;  // the segment's sequence began in an earlier run
+    int n_seg = 0;
+    load_q(w.b);
+    for (int64_t n = 0; n < count; ++n) {
+      const int valid = w.valid();
+      const int b_now = w.b;
+      const bool seq_end = w.tile == w.ntile - 1;
+      const bool seg_end = seq_end || n + 1 == count;
+      const int sc = (int)(n % kScaleStages);
+      if (!__all_sync(0xffffffffu, mbar_wait(&sc_full[sc], (uint32_t)(n / kScaleStages) & 1u, abort))) { ok = false; break; }
+      // a scale of zero (a row never written) counts as a tiny one
+      const float sigma = j < valid ? fmaxf(reinterpret_cast<const float*>(smem + S::OFF_SC)[sc * kTileTok + j], 0x1p-100f)
+                                    : 1.0f;
+      warp_arrive(&sc_empty[sc]);
+      const float lsig = __log2f(sigma), isig = __frcp_rn(sigma);
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[n & 1], (uint32_t)(n >> 1) & 1u, abort))) { ok = false; break; }
+      tc_fence_after();
+      float u[HW];
+      {
+        float lo[HW];
+        const uint32_t ts = t_lane + S::T_S + (uint32_t)(n & 1) * 2 * HB + wg * HW;
+        tmem_ld(ts, u);
+        tmem_ld(ts + HB, lo);
+#pragma unroll
+        for (int h = 0; h < HW; h += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(fh + wg * HW + h);
+          u[h + 0] = fmaf((u[h + 0] + lo[h + 0]) * sigma, f.x, lsig);
+          u[h + 1] = fmaf((u[h + 1] + lo[h + 1]) * sigma, f.y, lsig);
+          u[h + 2] = fmaf((u[h + 2] + lo[h + 2]) * sigma, f.z, lsig);
+          u[h + 3] = fmaf((u[h + 3] + lo[h + 3]) * sigma, f.w, lsig);
+        }
+        if (valid < kTileTok) {
+#pragma unroll
+          for (int h = 0; h < HW; ++h) u[h] = j < valid ? u[h] : -INFINITY;
+        }
+      }
+      // the tile's maximum per head: over the warp's tokens, then the warpgroup's
+      float mine = 0.0f;
+#pragma unroll
+      for (int h = 0; h < HW; ++h) {
+        const float r = redux_max(u[h]);
+        if (lane % HW == h) mine = r;
+      }
+      float* red_n = red + (((int)(n & 1) * 2 + wg) * 4) * HW;
+      if (lane < HW) red_n[quarter * HW + lane] = mine;
+      if (!__all_sync(0xffffffffu, mbar_rendezvous(&wg_bar[wg], meet, abort))) { ok = false; break; }
+      {
+        const int h = lane % HW;
+        float t = fmaxf(fmaxf(red_n[h], red_n[HW + h]), fmaxf(red_n[2 * HW + h], red_n[3 * HW + h]));
+        if (t == -INFINITY) t = 0.0f;
+        const float top = fmaxf(m_run, t);
+        const float a = fast_exp2(m_run - top), bt = fast_exp2(t - top);
+        m_run = top;
+        l_run *= a;
+        if (lane < HW) {
+          mt[lane] = t;
+          ab[lane] = a;
+          ab[HW + lane] = bt;
+        }
+        __syncwarp();
+        mine = bt;
+      }
+      // probabilities in units of 2^-8 of the tile's largest, their sum and digits
+      uint32_t hi[HW / 4], lo[HW / 4];
+#pragma unroll
+      for (int h = 0; h < HW; h += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(mt + h);
+        u[h + 0] = fast_exp2(u[h + 0] - t.x + 8.0f);
+        u[h + 1] = fast_exp2(u[h + 1] - t.y + 8.0f);
+        u[h + 2] = fast_exp2(u[h + 2] - t.z + 8.0f);
+        u[h + 3] = fast_exp2(u[h + 3] - t.w + 8.0f);
+        uint32_t a, b2, c, d;
+        split_digits(u[h + 0], u[h + 1], a, b2);
+        split_digits(u[h + 2], u[h + 3], c, d);
+        hi[h / 4] = a | (c << 16);
+        lo[h / 4] = b2 | (d << 16);
+      }
+      {
+        uint8_t* dst = smem + S::OFF_P + (wg * HW / 16) * (kTileTok * 16) + j * 16 + (wg * HW) % 16;
+        if constexpr (HW >= 16) {
+#pragma unroll
+          for (int i = 0; i < HW / 16; ++i) {
+            *reinterpret_cast<uint4*>(dst + i * (kTileTok * 16)) =
+                make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+            *reinterpret_cast<uint4*>(dst + S::P_BYTES + i * (kTileTok * 16)) =
+                make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+          }
+        } else {
+          *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(dst + S::P_BYTES) = make_uint2(lo[0], lo[1]);
+        }
+      }
+      if (j >= valid) {
+        // whatever lies past the sequence's end must not meet a zero
+        // probability as NaN: this warpgroup clears its half of the slabs
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        for (int g = wg; g < NL; g += 2) {
+          uint4* r = reinterpret_cast<uint4*>(smem + S::OFF_RING + (int)((n * NSLAB + 1 + g) % NS) * S::SLAB + j * 128);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) r[i] = z;
+        }
+      }
+      fence_proxy_async_shared();
+      warp_arrive(p_full);
+      // softmax sum: each lane ends with head lane % HW over the warp's tokens
+#pragma unroll
+      for (int h = 0; h < HW; ++h) u[h] *= isig;
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) {
+        if (o >= HW) {
+#pragma unroll
+          for (int h = 0; h < HW; ++h) u[h] += __shfl_xor_sync(0xffffffffu, u[h], o);
+        } else {
+          const bool up = (lane & o) != 0;
+#pragma unroll
+          for (int h = 0; h < o; ++h) {
+            const float give = up ? u[h] : u[h + o], keep = up ? u[h + o] : u[h];
+            u[h] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+          }
+        }
+      }
+      l_run = fmaf(u[0], mine, l_run);
+      if (n + 1 < count) {
+        w.next();
+        if (seg_end) load_q(w.b);  // the old query's last QK is done
+      }
+      // this tile's O^T into the registers, block by block as it is finished
+      bool good = true;
+#pragma unroll
+      for (int g = 0; g < NL; ++g) {
+        good = good && __all_sync(0xffffffffu, mbar_wait(&o_full[g], (uint32_t)n & 1u, abort));
+        if (!good) break;
+        tc_fence_after();
+        float o[HW];
+        tmem_ld(t_lane + S::T_O + g * HB + wg * HW, o);
+#pragma unroll
+        for (int h = 0; h < HW; h += 4) {
+          const float4 a = *reinterpret_cast<const float4*>(ab + h), bt = *reinterpret_cast<const float4*>(ab + HW + h);
+          acc[g][h + 0] = fmaf(acc[g][h + 0], a.x, o[h + 0] * bt.x);
+          acc[g][h + 1] = fmaf(acc[g][h + 1], a.y, o[h + 1] * bt.y);
+          acc[g][h + 2] = fmaf(acc[g][h + 2], a.z, o[h + 2] * bt.z);
+          acc[g][h + 3] = fmaf(acc[g][h + 3], a.w, o[h + 3] * bt.w);
+        }
+      }
+      if (!good) { ok = false; break; }
+      tc_fence_before();
+      warp_arrive(o_free);
+      if (!seg_end) continue;
+
+      // ------------------------------------------------ the segment's result
+      if (lane < HW) lred[(wg * 4 + quarter) * HW + lane] = l_run;
+      if (!__all_sync(0xffffffffu, mbar_rendezvous(&wg_bar[wg], meet, abort))) { ok = false; break; }
+      const int hl = lane % HW;
+      const float l = lred[(wg * 4 + 0) * HW + hl] + lred[(wg * 4 + 1) * HW + hl] + lred[(wg * 4 + 2) * HW + hl] +
+                      lred[(wg * 4 + 3) * HW + hl];
+      const int hb = h0 + wg * HW;  // first head of this warpgroup
+      if (!shared_front && seq_end) {
+        if (lane < HW) mt[lane] = 1.0f / l;
+        __syncwarp();
+        const bool odd = lane & 1;
+#pragma unroll
+        for (int h = 0; h < HW; h += 2) {
+          const float2 il = *reinterpret_cast<const float2*>(mt + h);
+          const int head = hb + h + (odd ? 1 : 0);
+          // lanes swap so that each stores two columns of one head
+          __nv_bfloat16* dst = out + ((int64_t)b_now * H + head) * R + quarter * 32 + (lane & ~1);
+#pragma unroll
+          for (int g = 0; g < NL; ++g) {
+            const float x = acc[g][h] * il.x, y = acc[g][h + 1] * il.y;
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? x : y, 1);
+            if (head < H) *reinterpret_cast<uint32_t*>(dst + g * 128) = odd ? pack_bf16x2(got, y) : pack_bf16x2(x, got);
+          }
+        }
+        __syncwarp();
+      } else {
+        const int64_t slot = (int64_t)blockIdx.x * 2 + (n_seg > 0 ? 1 : 0);
+        float* dst = ws_o + (slot * HB + wg * HW) * R + j;
+#pragma unroll
+        for (int h = 0; h < HW; ++h)
+          if (hb + h < H) {
+#pragma unroll
+            for (int g = 0; g < NL; ++g) dst[(int64_t)h * R + g * 128] = acc[g][h];
+          }
+        if (quarter == 0 && lane < HW) ws_ml[slot * HB + wg * HW + lane] = make_float2(m_run, l);
+      }
+#pragma unroll
+      for (int g = 0; g < NL; ++g)
+#pragma unroll
+        for (int h = 0; h < HW; ++h) acc[g][h] = 0.0f;
+      m_run = -INFINITY;
+      l_run = 0.0f;
+      shared_front = false;
+      ++n_seg;
+    }
+    if (!ok) raise_abort(abort, status, kStatusTimeout);
+  }
+
+  tc_fence_before();
   __syncthreads();
-  float mt = -INFINITY, lt = 0.0f;
-  for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, sm[w]);
-  for (int w = 0; w < kWarps; ++w) lt += sm[w] == -INFINITY ? 0.0f : sl[w] * exp2f(sm[w] - mt);
-  for (int i = threadIdx.x; i < R; i += kWarps * 32) {
-    float acc = 0.0f;
-    for (int w = 0; w < kWarps; ++w) acc += sm[w] == -INFINITY ? 0.0f : so[w][i] * exp2f(sm[w] - mt);
-    out[((int64_t)b * H + h) * R + i] = __float2bfloat16_rn(lt > 0.0f ? acc / lt : 0.0f);
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::T_COLS);
   }
+}
+
+// Sequences shared by several runs (their partials: sum_i 2^(m_i - M) O_i /
+// sum_i 2^(m_i - M) l_i), and empty ones (zero rows).  A CTA per (sequence,
+// head), its warps taking every 8th partial; with many sequences (few
+// partials each) a warp per head.
+constexpr int kCombineWarps = 8;
+
+template <int R, bool kWarpPerHead>
+__global__ void __launch_bounds__(kCombineWarps * 32)
+    combine_kernel(const int32_t* __restrict__ prefix, int B, int H, int HB, int runs,
+                   const float* __restrict__ ws_o, const float2* __restrict__ ws_ml, __nv_bfloat16* __restrict__ out) {
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr int V = R / 128;  // float4 per lane
+  const int warp = (int)warp_id(), lane = (int)lane_id();
+  const int b = blockIdx.x, h = kWarpPerHead ? blockIdx.y * kCombineWarps + warp : blockIdx.y;
+  const int64_t t0 = prefix[b], t1 = prefix[b + 1], T = prefix[B];
+  __nv_bfloat16* dst = out + ((int64_t)b * H + h) * R + lane * 4;
+  if (t0 == t1) {
+    if (h < H && (kWarpPerHead || warp == 0)) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) *reinterpret_cast<uint2*>(dst + v * 128) = make_uint2(0, 0);
+    }
+    return;
+  }
+  const int i0 = run_of(t0, T, runs), i1 = run_of(t1 - 1, T, runs);
+  if (i0 == i1) return;  // written whole
+  if (kWarpPerHead && h >= H) return;
+  const int64_t cta0 = (int64_t)(h / HB) * runs, hl = h % HB;
+  // the first run's segment of this sequence is its last one: its second
+  // slot, unless the run also begins there
+  auto slot_of = [&](int i) { return (cta0 + i) * 2 + (i == i0 && run_start(i, T, runs) != t0 ? 1 : 0); };
+  float m = -INFINITY, l = 0.0f;
+  float4 o[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int kStep = kWarpPerHead ? 1 : kCombineWarps;
+#pragma unroll 4
+  for (int i = i0 + (kWarpPerHead ? 0 : warp); i <= i1; i += kStep) {
+    // a run between i0 and i1 may be empty only when there are fewer tiles
+    // than runs; it then wrote nothing
+    if (run_start(i, T, runs) == run_start(i + 1, T, runs)) continue;
+    const int64_t s = slot_of(i) * HB + hl;
+    const float2 ml = ws_ml[s];
+    const float mn = fmaxf(m, ml.x), a = exp2f(m - mn), c = exp2f(ml.x - mn);
+    m = mn;
+    l = l * a + ml.y * c;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float4 x = *reinterpret_cast<const float4*>(ws_o + s * R + v * 128 + lane * 4);
+      o[v].x = o[v].x * a + x.x * c;
+      o[v].y = o[v].y * a + x.y * c;
+      o[v].z = o[v].z * a + x.z * c;
+      o[v].w = o[v].w * a + x.w * c;
+    }
+  }
+  if constexpr (!kWarpPerHead) {
+    __shared__ float sm[kCombineWarps], sl[kCombineWarps];
+    __shared__ float4 so[kCombineWarps][R / 4];
+    if (lane == 0) {
+      sm[warp] = m;
+      sl[warp] = l;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) so[warp][v * 32 + lane] = o[v];
+    __syncthreads();
+    if (warp >= V) return;  // warp v merges columns [128 v, 128 v + 128)
+    float top = -INFINITY, den = 0.0f;
+    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < kCombineWarps; ++i) top = fmaxf(top, sm[i]);
+    for (int i = 0; i < kCombineWarps; ++i) {
+      if (sm[i] == -INFINITY) continue;  // no partial
+      const float c = exp2f(sm[i] - top);
+      const float4 x = so[i][warp * 32 + lane];
+      den += sl[i] * c;
+      r.x += x.x * c;
+      r.y += x.y * c;
+      r.z += x.z * c;
+      r.w += x.w * c;
+    }
+    const float inv = 1.0f / den;
+    *reinterpret_cast<uint2*>(dst + warp * 128) =
+        make_uint2(pack_bf16x2(r.x * inv, r.y * inv), pack_bf16x2(r.z * inv, r.w * inv));
+  } else {
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      *reinterpret_cast<uint2*>(dst + v * 128) =
+          make_uint2(pack_bf16x2(o[v].x * inv, o[v].y * inv), pack_bf16x2(o[v].z * inv, o[v].w * inv));
+  }
+}
+
+// The scratch: the prefix array, then every CTA's two partials.  One size for
+// every call (128 KB a partial at 64 heads x 512 columns), so that captured
+// calls keep their addresses.
+size_t scratch_bytes(int sm) {
+  const size_t partials = (size_t)sm * 2 * kMaxHeadsPerCta;
+  return (kMaxSeqs + 64) * sizeof(int32_t) + partials * (512 * sizeof(float) + sizeof(float2));
+}
+
+template <int R, int P, int HB>
+int launch(dsb_ctx* ctx, const void* q_lat, const void* q_rope, const void* cache, const float* scales,
+           int64_t n_blocks, const int32_t* block_table, int max_blocks, const int32_t* seq_lens, int B, int H,
+           float softmax_scale, void* out) {
+  using S = Shape<R, P, HB>;
+  CUtensorMap map_lat, map_rope;
+  const uint64_t rows = (uint64_t)n_blocks * kPageTok, pitch = R + 2 * P;
+  int rc = make_tmap_2d(ctx, &map_lat, cache, CU_TENSOR_MAP_DATA_TYPE_UINT8, pitch, rows, pitch, 128, kPageTok,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+  if (rc != DSB_OK) return rc;
+  rc = make_tmap_2d(ctx, &map_rope, cache, CU_TENSOR_MAP_DATA_TYPE_UINT8, pitch, rows, pitch, P * 2, kPageTok,
+                    P == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+  if (rc != DSB_OK) return rc;
+  const int groups = (H + HB - 1) / HB;
+  const int runs = std::max(1, ctx->sm_count / groups);
+  auto* prefix = static_cast<int32_t*>(ctx->mla8);
+  auto* ws_ml = reinterpret_cast<float2*>(prefix + kMaxSeqs + 64);
+  auto* ws_o = reinterpret_cast<float*>(ws_ml + (size_t)ctx->sm_count * 2 * kMaxHeadsPerCta);
+  auto kern = decode_fp8_kernel<R, P, HB>;
+  static std::atomic<bool> attr_set[kMaxDevices];
+  if (rc = smem_attr_once(ctx, kern, S::SMEM_BYTES, attr_set); rc != DSB_OK) return rc;
+  DSB_CUDA_TRY(ctx, launch_pdl(kern, dim3((unsigned)(groups * runs)), kThreads, S::SMEM_BYTES, ctx->stream, map_lat,
+                               map_rope, static_cast<const __nv_bfloat16*>(q_lat),
+                               static_cast<const __nv_bfloat16*>(q_rope), scales, n_blocks, block_table, max_blocks,
+                               seq_lens, B, H, runs, softmax_scale * 1.4426950408889634f,
+                               static_cast<__nv_bfloat16*>(out), ws_o, ws_ml, prefix, ctx->d_status));
+  auto combine = [&](auto kernel, unsigned y) {
+    return launch_pdl(kernel, dim3((unsigned)B, y), kCombineWarps * 32, 0, ctx->stream, prefix, B, H, HB, runs, ws_o,
+                      ws_ml, static_cast<__nv_bfloat16*>(out));
+  };
+  // a sequence has about runs / B partials
+  if (B >= 32) DSB_CUDA_TRY(ctx, combine(combine_kernel<R, true>, (unsigned)((H + kCombineWarps - 1) / kCombineWarps)));
+  else DSB_CUDA_TRY(ctx, combine(combine_kernel<R, false>, (unsigned)H));
+  ctx->stats.kernel_launches += 2;
+  ctx->stats.mla_calls++;
+  return DSB_OK;
 }
 
 }  // namespace
@@ -108,24 +872,25 @@ extern "C" int dsb_mla_decode_fp8(dsb_ctx* ctx, const void* q_lat, const void* q
     return fail(ctx, DSB_EINVAL, "dsb_mla_decode_fp8: null pointer argument");
   if (!cache_shape_ok(R, P))
     return fail(ctx, DSB_EUNSUPPORTED, "dsb_mla_decode_fp8: (R, P) = (%d, %d) not supported", R, P);
-  if (B <= 0 || H <= 0 || H > 128 || max_blocks <= 0 || n_blocks <= 0 || n_blocks >= (1 << 25) ||
+  if (B <= 0 || B > kMaxSeqs || H <= 0 || H > 128 || max_blocks <= 0 || n_blocks <= 0 || n_blocks >= (1 << 25) ||
       !std::isfinite(softmax_scale))
     return fail(ctx, DSB_EINVAL, "dsb_mla_decode_fp8: bad arguments B=%d H=%d max_blocks=%d n_blocks=%lld scale=%g", B,
                 H, max_blocks, (long long)n_blocks, softmax_scale);
-  if ((reinterpret_cast<uintptr_t>(q_lat) | reinterpret_cast<uintptr_t>(q_rope) |
+  if ((reinterpret_cast<uintptr_t>(q_lat) | reinterpret_cast<uintptr_t>(q_rope) | reinterpret_cast<uintptr_t>(scales) |
        reinterpret_cast<uintptr_t>(out_lat) | reinterpret_cast<uintptr_t>(cache)) & 15u)
     return fail(ctx, DSB_EINVAL, "dsb_mla_decode_fp8: pointers must be 16-byte aligned");
   DeviceScope scope(ctx->device);
   if (!scope.ok) return fail(ctx, DSB_ECUDA, "dsb_mla_decode_fp8: cudaSetDevice(%d) failed", ctx->device);
-  auto run = [&](auto kernel) {
-    DSB_CUDA_TRY(ctx, launch_pdl(kernel, dim3((unsigned)B, (unsigned)H), kWarps * 32, 0, ctx->stream,
-                                 static_cast<const __nv_bfloat16*>(q_lat), static_cast<const __nv_bfloat16*>(q_rope),
-                                 static_cast<const uint8_t*>(cache), scales, n_blocks, block_table, max_blocks,
-                                 seq_lens, H, softmax_scale * 1.4426950408889634f,
-                                 static_cast<__nv_bfloat16*>(out_lat), ctx->d_status));
-    ctx->stats.kernel_launches++;
-    ctx->stats.mla_calls++;
-    return (int)DSB_OK;
+  if (ctx->mla8 == nullptr) {
+    const size_t need = scratch_bytes(ctx->sm_count);
+    if (int rc = ensure_buffer(ctx, &ctx->mla8, &ctx->mla8_bytes, need, need, "dsb_mla_decode_fp8"); rc != DSB_OK)
+      return rc;
+  }
+  auto run = [&](auto f) {
+    return f(ctx, q_lat, q_rope, cache, scales, n_blocks, block_table, max_blocks, seq_lens, B, H, softmax_scale,
+             out_lat);
   };
-  return R == 512 ? run(decode_fp8_kernel<512, 64>) : run(decode_fp8_kernel<128, 32>);
+  // the fewest columns that hold the heads: a tile's MMA time grows with them
+  if (R == 512) return H <= 16 ? run(launch<512, 64, 16>) : H <= 32 ? run(launch<512, 64, 32>) : run(launch<512, 64, 64>);
+  return H <= 16 ? run(launch<128, 32, 16>) : H <= 32 ? run(launch<128, 32, 32>) : run(launch<128, 32, 64>);
 }

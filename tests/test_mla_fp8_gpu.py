@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import mla_fp8_ref as ref
-from deepseek_cpp_infer_b200 import DSB_EINVAL, DSB_EUNSUPPORTED, Context, DsbError
+from deepseek_cpp_infer_b200 import DSB_EINVAL, DSB_EUNSUPPORTED as DSB_UNSUP, Context, DsbError
 
 pytestmark = pytest.mark.gpu
 
@@ -432,38 +432,56 @@ def test_read_bad_pages_are_reported(gpu_ctx):
 
 
 def test_refusals(gpu_ctx):
+    """At the C entry points (the bindings' own checks come before some of these: they raise ValueError)."""
     import torch
 
     lens = [100]
     q_lat, q_rope, cache, scales, table, scale = decode_inputs(lens, 16, BIG, seed=1)
     sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
     out = torch.empty_like(q_lat)
-
-    def refused(code, f, *a, **k):
-        with pytest.raises(DsbError) as e:
-            f(*a, **k)
-        assert e.value.code == code
-
-    dec = gpu_ctx.mla_decode_fp8
-    refused(DSB_EINVAL, dec, q_lat, q_rope, cache, scales, table, None, scale, out)
-    refused(DSB_EINVAL, dec, q_lat, q_rope, cache, scales, table, sl, float("nan"), out)
-    refused(DSB_EINVAL, dec, q_lat, q_rope, cache, scales, table, sl, float("inf"), out)
-    refused(DSB_EUNSUPPORTED, dec, q_lat[..., :256], q_rope, cache, scales, table, sl, scale, out)
-    refused(DSB_EINVAL, dec, q_lat.repeat(1, 9, 1), q_rope, cache, scales, table, sl, scale, out)  # 144 heads
-    refused(DSB_EINVAL, dec, q_lat, q_rope, cache, scales, table, sl, scale, out.view(-1)[1:])
-    kv, w, q = append_case(1, 16, BIG, seed=1)
-    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
-    app = gpu_ctx.kv_norm_rope_append_fp8
-    refused(DSB_EUNSUPPORTED, app, kv, w, q, pos, table, 16, 128, 256, 64, EPS, THETA, cache, scales, q_rope)
-    refused(DSB_EINVAL, app, kv, w, q, pos, table, 16, 100, 512, 64, EPS, THETA, cache, scales, q_rope)
-    refused(DSB_EINVAL, app, kv, w, q, pos, table, 16, 128, 512, 64, EPS, 0.0, cache, scales, q_rope)
-    refused(DSB_EINVAL, app, kv, w, q, pos, table, 17, 128, 512, 64, EPS, THETA, cache, scales, q_rope)  # q too narrow
-    refused(DSB_EINVAL, app, kv.repeat(2, 1), w, q.repeat(2, 1), pos, table, 16, 128, 512, 64, EPS, THETA, cache,
-            scales, q_rope)  # two rows, one sequence, no seq_ids
-    lat, rope = torch.empty(100, 512, dtype=torch.bfloat16, device="cuda"), torch.empty(100, 64, dtype=torch.bfloat16, device="cuda")
+    kv, w, q = append_case(2, 16, BIG, seed=1)
+    pos = torch.zeros(2, dtype=torch.int32, device="cuda")
+    qr2 = torch.empty(2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    lat = torch.empty(100, 512, dtype=torch.bfloat16, device="cuda")
+    rope = torch.empty(100, 64, dtype=torch.bfloat16, device="cuda")
     cu = torch.tensor([0, 100], dtype=torch.int32, device="cuda")
-    read = gpu_ctx.mla_cache_read_fp8
-    refused(DSB_EUNSUPPORTED, read, cache, scales, table, cu, lat[:, :256], rope)
-    refused(DSB_EINVAL, read, cache, scales, table, None, lat, rope)
-    refused(DSB_EINVAL, read, cache, scales, table, cu, torch.empty(100, 516, dtype=torch.bfloat16, device="cuda")[:, :512], rope)
+
+    def p(t):
+        return t.data_ptr()
+
+    l, h, n = gpu_ctx._l, gpu_ctx.h, cache.shape[0]
+    dec = dict(ctx=h, q_lat=p(q_lat), q_rope=p(q_rope), cache=p(cache), scales=p(scales), n_blocks=n, table=p(table),
+               max_blocks=table.shape[1], lens=p(sl), B=1, H=16, R=512, P=64, scale=scale, out=p(out))
+    app = dict(ctx=h, kv=p(kv), ld_kv=kv.stride(0), w=p(w), q=p(q), ldq=q.stride(0), pos=p(pos), seq=None,
+               table=p(table), n_seqs=2, max_blocks=table.shape[1], B=2, H=16, nope=128, R=512, P=64, eps=EPS,
+               theta=THETA, cache=p(cache), scales=p(scales), n_blocks=n, q_rope=p(qr2))
+    read = dict(ctx=h, cache=p(cache), scales=p(scales), n_blocks=n, table=p(table), max_blocks=table.shape[1],
+                cu=p(cu), B=1, T=100, R=512, P=64, lat=p(lat), ld_lat=512, rope=p(rope), ld_rope=64)
+    for f, args, bad in (
+            (l.dsb_mla_decode_fp8, dec,
+             [(DSB_EINVAL, k, None) for k in ("ctx", "q_lat", "q_rope", "cache", "scales", "table", "lens", "out")]
+             + [(DSB_EINVAL, "scale", float("nan")), (DSB_EINVAL, "scale", float("inf")), (DSB_UNSUP, "R", 256),
+                (DSB_UNSUP, "P", 32), (DSB_EINVAL, "H", 0), (DSB_EINVAL, "H", 129), (DSB_EINVAL, "B", 0),
+                (DSB_EINVAL, "max_blocks", 0), (DSB_EINVAL, "n_blocks", 0), (DSB_EINVAL, "n_blocks", 1 << 25),
+                (DSB_EINVAL, "out", p(out) + 2), (DSB_EINVAL, "q_lat", p(q_lat) + 8), (DSB_EINVAL, "cache", p(cache) + 1)]),
+            (l.dsb_kv_norm_rope_append_fp8, app,
+             [(DSB_EINVAL, k, None) for k in ("ctx", "kv", "w", "q", "pos", "table", "cache", "scales", "q_rope")]
+             + [(DSB_UNSUP, "R", 256), (DSB_UNSUP, "P", 128), (DSB_EINVAL, "nope", 100), (DSB_EINVAL, "nope", -8),
+                (DSB_EINVAL, "theta", 0.0), (DSB_EINVAL, "theta", float("inf")), (DSB_EINVAL, "eps", -1.0),
+                (DSB_EINVAL, "ldq", 16 * 192 - 8), (DSB_EINVAL, "ld_kv", 575), (DSB_EINVAL, "ld_kv", 578),
+                (DSB_EINVAL, "n_seqs", 1), (DSB_EINVAL, "H", 0), (DSB_EINVAL, "B", 0), (DSB_EINVAL, "kv", p(kv) + 4),
+                (DSB_EINVAL, "n_blocks", 0)]),
+            (l.dsb_mla_cache_read_fp8, read,
+             [(DSB_EINVAL, k, None) for k in ("ctx", "cache", "scales", "table", "cu")]
+             + [(DSB_UNSUP, "R", 64), (DSB_EINVAL, "T", -1), (DSB_EINVAL, "B", 0), (DSB_EINVAL, "ld_lat", 504),
+                (DSB_EINVAL, "ld_lat", 516), (DSB_EINVAL, "ld_rope", 56), (DSB_EINVAL, "lat", p(lat) + 2)])):
+        for code, k, v in bad:
+            assert f(*{**args, k: v}.values()) == code, (f.__name__, k, v)
+    for args in ((q_lat, q_rope, cache, scales, table, sl.long(), scale, out),
+                 (q_lat.transpose(1, 2).contiguous().transpose(1, 2), q_rope, cache, scales, table, sl, scale, out),
+                 (q_lat, q_rope, cache, scales[:1], table, sl, scale, out),
+                 (q_lat, q_rope, cache, scales, table.cpu(), sl, scale, out),
+                 (q_lat.float(), q_rope, cache, scales, table, sl, scale, out)):
+        with pytest.raises(ValueError):
+            gpu_ctx.mla_decode_fp8(*args)
     gpu_ctx.sync()

@@ -251,10 +251,22 @@ def test_refusals(gpu_ctx):
 
     refused(DSB_EUNSUPPORTED, qn[..., :64], qr, kn[..., :64], kr, v)
     refused(DSB_EUNSUPPORTED, qn, qr, kn, kr, v[..., :64])
-    refused(DSB_EINVAL, qn.reshape(-1)[1:10 * 2 * 128 - 127].unfold(0, 128, 128)[:18].view(9, 2, 128), qr, kn, kr, v)
+    import torch
+
+    shifted = torch.empty(10 * 2 * 128 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(10, 2, 128)  # 2-byte aligned
+    refused(DSB_EINVAL, shifted, qr, kn, kr, v)
+    odd = torch.empty(10, 2, 132, dtype=torch.bfloat16, device="cuda")[..., :128]  # head pitch 132
+    refused(DSB_EINVAL, qn, qr, odd, kr, v)
     with pytest.raises(DsbError) as e:
-        gpu_ctx.mla_prefill(qn, qr, kn, kr, v, cu_of([10]), cu_of([10]), 10, float("nan"), kn)
+        gpu_ctx.mla_prefill(qn, qr, kn, kr, v, cu_of([10]), cu_of([10]), 10, float("nan"),
+                            torch.empty(10, 2, 128, dtype=torch.bfloat16, device="cuda"))
     assert e.value.code == DSB_EINVAL
+    with pytest.raises(ValueError):  # the binding: strided innermost dimension, wrong type
+        gpu_ctx.mla_prefill(qn.transpose(1, 2).contiguous().transpose(1, 2), qr, kn, kr, v, cu_of([10]), cu_of([10]), 10,
+                            scale, torch.empty(10, 2, 128, dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(ValueError):
+        gpu_ctx.mla_prefill(qn, qr, kn, kr, v.half(), cu_of([10]), cu_of([10]), 10, scale,
+                            torch.empty(10, 2, 128, dtype=torch.bfloat16, device="cuda"))
     gpu_ctx.sync()
 
 
@@ -277,6 +289,7 @@ def test_prompt_then_decode(gpu_ctx, H, dims, R):
         return torch.randn(*s, generator=g, device="cuda") * std
 
     w_uk, w_uv = r(H, nope, R, std=R ** -0.5).bfloat16(), r(H, vd, R, std=R ** -0.5).bfloat16()
+    w_kv = torch.cat([w_uk, w_uv], 1).reshape(H * (nope + vd), R).contiguous()
     w_norm = 1 + 0.1 * r(R)
     scale = 1 / math.sqrt(nope + P)
     total, chunks, n_new = [150, 67], [[70, 60], [80, 7]], 3
@@ -298,7 +311,7 @@ def test_prompt_then_decode(gpu_ctx, H, dims, R):
         return q.view(T, H, nope + P)[..., :nope], q_rope
 
     def absorb(q_nope):
-        return torch.einsum("thn,hnr->thr", q_nope.float(), w_uk.float()).bfloat16()
+        return torch.einsum("thn,hnr->thr", q_nope.float(), w_uk.float()).bfloat16().contiguous()
 
     for lens in chunks:
         q_nope, q_rope = append(lens)
@@ -307,7 +320,6 @@ def test_prompt_then_decode(gpu_ctx, H, dims, R):
         rope = torch.empty(T, P, dtype=torch.bfloat16, device="cuda")
         gpu_ctx.mla_cache_read_fp8(cache, scales, table, cu_of(have), lat, rope)
         kv = torch.empty(T, H * (nope + vd), dtype=torch.bfloat16, device="cuda")
-        w_kv = torch.cat([w_uk, w_uv], 1).reshape(H * (nope + vd), R).contiguous()
         gpu_ctx.linear(w_kv, lat, kv, M=H * (nope + vd), K=R)
         kv = kv.view(T, H, nope + vd)
         x = (q_nope, q_rope, kv[..., :nope], rope, kv[..., nope:], scale)
