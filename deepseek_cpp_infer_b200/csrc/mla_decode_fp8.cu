@@ -28,8 +28,8 @@
 // device.  A run's first and last sequences may be shared with its neighbours:
 // such segments go to fp32 partials that combine_kernel merges.
 //
-// Roles (10 warps): 8 softmax / accumulate warps, two warpgroups with half of
-// the heads each (thread = token for S^T, thread = latent column for O^T), a
+// Roles (10 warps): 8 softmax / accumulate warps, warpgroups with their
+// share of the heads each (thread = token for S^T, thread = latent column for O^T), a
 // TMA warp and an MMA warp.  Shared memory is a ring of 128-token x 128-byte
 // slabs (R / 128 of latents and one of rope keys per tile): a slab serves QK
 // and, as soon as its block of O^T is done, is free again, so that at 64 heads
@@ -51,8 +51,6 @@ namespace dsb {
 namespace {
 
 constexpr int kTileTok = 128;       // tokens per tile: MMA M
-constexpr int kSmWarps = 8;         // softmax / accumulate warps
-constexpr int kThreads = (kSmWarps + 2) * 32;
 constexpr int kMaxHeadsPerCta = 64;
 constexpr int kMaxSeqs = 65536;     // prefix array in the scratch
 constexpr int kScaleStages = 4;
@@ -61,7 +59,10 @@ template <int R, int P, int HB>
 struct Shape {
   static constexpr int NL = R / 128;                 // latent slabs per tile
   static constexpr int NSLAB = NL + 1;               // + rope
-  static constexpr int HW = HB / 2;                  // heads per warpgroup
+  static constexpr int NWG = HB == 64 ? 4 : 2;       // softmax warpgroups
+  static constexpr int SM_WARPS = NWG * 4;
+  static constexpr int THREADS = (SM_WARPS + 2) * 32;  // + TMA and MMA
+  static constexpr int HW = HB / NWG;                // heads per warpgroup
   static constexpr int SLAB = kTileTok * 128;        // bytes
   static constexpr int NS = HB == 16 ? 12 : HB == 32 || NL == 1 ? 10 : 8;  // ring slots: what fits
   // slabs of tile n + 1's QK issued before tile n's PV: all when two tiles
@@ -76,14 +77,13 @@ struct Shape {
   static constexpr int OFF_QR = OFF_Q8 + Q8_BYTES;
   static constexpr int OFF_P = OFF_QR + QR_BYTES;
   static constexpr int OFF_SC = OFF_P + 2 * P_BYTES;                     // [stages][128] token scales
-  static constexpr int OFF_RED = OFF_SC + kScaleStages * kTileTok * 4;   // [2 parity][2 wg][4 warps][HW] maxima
-  static constexpr int OFF_LRED = OFF_RED + 2 * 2 * 4 * HW * 4;          // [2 wg][4 warps][HW] sums
-  static constexpr int OFF_AB = OFF_LRED + 2 * 4 * HW * 4;               // per warp [2][HW]: old and tile weights
-  static constexpr int OFF_MT = OFF_AB + kSmWarps * 2 * HW * 4;          // per warp [HW]: tile maxima (or 1 / sums)
-  static constexpr int OFF_FH = OFF_MT + kSmWarps * HW * 4;              // [HB] a_h * scale * log2(e)
-  static constexpr int NBAR = 2 * NS + 2 + NL + 6 + 2 * kScaleStages;
+  static constexpr int OFF_RED = OFF_SC + kScaleStages * kTileTok * 4;   // [2 parity][NWG][4 warps][HW] maxima
+  static constexpr int OFF_LRED = OFF_RED + 2 * 4 * HB * 4;              // [NWG][4 warps][HW] sums
+  static constexpr int OFF_MT = OFF_LRED + 4 * HB * 4;                   // per warp [HW]: references (or 1 / sums)
+  static constexpr int OFF_FH = OFF_MT + 4 * HB * 4;              // [HB] a_h * scale * log2(e)
+  static constexpr int NBAR = 2 * NS + 2 + 5 + NWG + 2 * kScaleStages;
   static constexpr int OFF_BAR = (OFF_FH + HB * 4 + 7) / 8 * 8;
-  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;                    // tmem base, abort flags, scan, start
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;                    // tmem base, abort flags, start, scan
   static constexpr int SMEM_BYTES = OFF_MISC + 128 + 1024;               // + alignment slack
   static_assert(SMEM_BYTES <= 232448, "shared memory");
   static_assert(OFF_Q8 % 1024 == 0 && OFF_QR % 1024 == 0 && OFF_P % 128 == 0 && OFF_SC % 16 == 0, "alignment");
@@ -122,15 +122,12 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// N columns of this thread's TMEM lane; tmem_ld_wait() before their use.
 template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[N]) {
-  uint32_t r[N];
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
   if constexpr (N == 32) tmem_ld32(taddr, r);
   else if constexpr (N == 16) tmem_ld16(taddr, r);
   else tmem_ld8(taddr, r);
-  tmem_ld_wait();
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 __device__ __forceinline__ bool bad_len(int len, int max_blocks) {
@@ -167,13 +164,39 @@ struct Walk {
   __device__ int valid() const { return min(kTileTok, len - tile * kTileTok); }  // tokens of this tile
 };
 
+// A position in the ring: slot and phase parity.
+template <int NS>
+struct Cursor {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ void step(int k) {
+    slot += k;
+    if (slot >= NS) {
+      slot -= NS;
+      phase ^= 1u;
+    }
+  }
+  __device__ Cursor plus(int k) const {
+    Cursor c = *this;
+    c.step(k);
+    return c;
+  }
+};
+
+__device__ __forceinline__ void tmem_ld1(uint32_t taddr, uint32_t& r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
+}
+
 // First tile of run i of n over T tiles.
 __device__ __forceinline__ int64_t run_start(int64_t i, int64_t T, int n) { return i * T / n; }
 // The run that holds tile t.
 __device__ __forceinline__ int run_of(int64_t t, int64_t T, int n) { return (int)(((t + 1) * n - 1) / T); }
 
 template <int R, int P, int HB>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     decode_fp8_kernel(const __grid_constant__ CUtensorMap map_lat, const __grid_constant__ CUtensorMap map_rope,
                       const __nv_bfloat16* __restrict__ q_lat, const __nv_bfloat16* __restrict__ q_rope,
                       const float* __restrict__ scales, int64_t n_blocks, const int32_t* __restrict__ block_table,
@@ -181,28 +204,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                       __nv_bfloat16* __restrict__ out, float* __restrict__ ws_o, float2* __restrict__ ws_ml,
                       int32_t* __restrict__ prefix, int* __restrict__ status) {
   using S = Shape<R, P, HB>;
-  constexpr int NL = S::NL, NS = S::NS, HW = S::HW, NSLAB = S::NSLAB;
+  constexpr int NL = S::NL, NS = S::NS, HW = S::HW, NSLAB = S::NSLAB, NWG = S::NWG;
+  constexpr int kSmWarps = S::SM_WARPS, kThreads = S::THREADS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::OFF_BAR);
   uint64_t* full = bars;                     // [NS] slab landed
   uint64_t* empty = full + NS;               // [NS] slab's last MMA done
   uint64_t* s_full = empty + NS;             // [2] scores of a tile ready
-  uint64_t* o_full = s_full + 2;             // [NL] a block of the tile's O^T ready
-  uint64_t* p_full = o_full + NL;            // probabilities of a tile written
-  uint64_t* o_free = p_full + 1;             // O^T of a tile taken into registers
+  uint64_t* pv_done = s_full + 2;            // a tile's PV done
+  uint64_t* p_full = pv_done + 1;            // probabilities of a tile written
+  uint64_t* o_free = p_full + 1;             // O^T of a segment read
   uint64_t* q_ready = o_free + 1;            // query digits of a segment written
-  uint64_t* wg_bar = q_ready + 1;            // [2] rendezvous of a warpgroup
-  uint64_t* sc_full = wg_bar + 2;            // [stages] token scales landed
+  uint64_t* wg_bar = q_ready + 1;            // [NWG] rendezvous of a warpgroup
+  uint64_t* sc_full = wg_bar + NWG;           // [stages] token scales landed
   uint64_t* sc_empty = sc_full + kScaleStages;
   uint64_t* drain = sc_empty + kScaleStages;  // every MMA issued is done
   uint32_t* misc = reinterpret_cast<uint32_t*>(smem + S::OFF_MISC);
   volatile int* abort = reinterpret_cast<volatile int*>(misc + 1);
   volatile int* no_abort = reinterpret_cast<volatile int*>(misc + 2);  // never raised: for drain waits
   int* start = reinterpret_cast<int*>(misc + 3);                       // sequence and tile of the run's start
-  int* scan = reinterpret_cast<int*>(misc + 8);                        // [10] warp totals
+  int* scan = reinterpret_cast<int*>(misc + 8);                        // [20] warp totals, at most
 
-  const int warp = (int)warp_id(), lane = (int)lane_id();
+  // warp-uniform for the compiler, so that the MMA and TMA operands stay in
+  // uniform registers
+  const int warp = __shfl_sync(0xffffffffu, (int)warp_id(), 0), lane = (int)lane_id();
   const int hg = blockIdx.x / runs, run = blockIdx.x % runs;  // head group and run
   constexpr int kTmaWarp = kSmWarps, kMmaWarp = kSmWarps + 1;
 
@@ -211,11 +237,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&wg_bar[i], kSmWarps / 2);
-    }
-    for (int i = 0; i < NL; ++i) mbar_init(&o_full[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
+    for (int i = 0; i < NWG; ++i) mbar_init(&wg_bar[i], 4);
+    mbar_init(pv_done, 1);
     mbar_init(p_full, kSmWarps);
     mbar_init(o_free, kSmWarps);
     mbar_init(q_ready, kSmWarps);
@@ -240,7 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
 
   // Tiles before each thread's share of the sequences, and this CTA's run.
-  int64_t run0, count;
+  int64_t run0;
+  int count;
   {
     const int per = (B + kThreads - 1) / kThreads;
     const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
@@ -267,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       T += scan[w];
     }
     run0 = run_start(run, T, runs);
-    count = run_start(run + 1, T, runs) - run0;
+    count = (int)(run_start(run + 1, T, runs) - run0);
     if (count > 0 && run0 >= before && run0 < before + mine) {
       int t = before, b = b0;
       for (;; ++b) {
@@ -297,44 +322,57 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ TMA producer
     // Slab order per tile: rope, latents 0 .. NL - 1 (the rope slab is free
     // again after QK, so its slot goes to the next tile's slab first).
-    if (lane == 0 && count > 0) {
+    if (count > 0) {
       const uint64_t policy = l2_policy_evict_first();
-      int it = 0;  // slabs issued
-      int nsc = 0; // scale stages issued
+      int it = 0;   // slabs issued
+      Cursor<NS> at_slab;
+      int nsc = 0;  // scale stages issued
+      int pages = 0, at = 32;  // page ids of the next 16 tiles of the sequence, two lanes a tile
       bool ok = true;
-      for (int64_t n = 0; ok && n < count; ++n) {
+      for (int n = 0; ok && n < count; ++n) {
         if (n > 0) w.next();
-        const int np = w.valid() > kPageTok ? 2 : 1;
-        int page[2] = {0, 0};
-        for (int p = 0; p < np; ++p) {
-          page[p] = block_table[(int64_t)w.b * max_blocks + w.tile * 2 + p];
-          if (page[p] < 0 || page[p] >= n_blocks) {  // read some page instead, and report it
-            page[p] = 0;
-            atomicCAS(status, 0, kStatusBadInput);
+        if (at == 32 || w.tile == 0) {
+          const int p = w.tile * 2 + lane;
+          pages = 0;
+          if (p * kPageTok < w.len) {
+            pages = block_table[(int64_t)w.b * max_blocks + p];
+            if (pages < 0 || pages >= n_blocks) {  // read some page instead, and report it
+              pages = 0;
+              atomicCAS(status, 0, kStatusBadInput);
+            }
           }
+          at = 0;
         }
-        const int sc = (int)(n % kScaleStages);
-        if (n >= kScaleStages && !mbar_wait(&sc_empty[sc], (uint32_t)(n / kScaleStages - 1) & 1u, abort)) {
+        const int np = w.valid() > kPageTok ? 2 : 1;
+        const int page[2] = {__shfl_sync(0xffffffffu, pages, at), __shfl_sync(0xffffffffu, pages, at + 1)};
+        at += 2;
+        const int sc = n % kScaleStages;
+        if (n >= kScaleStages &&
+            !__all_sync(0xffffffffu, mbar_wait(&sc_empty[sc], (uint32_t)(n / kScaleStages - 1) & 1u, abort))) {
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(&sc_full[sc], np * kPageTok * 4);
-        for (int p = 0; p < np; ++p)
-          bulk_load(smem + S::OFF_SC + (sc * kTileTok + p * kPageTok) * 4, scales + (int64_t)page[p] * kPageTok,
-                    kPageTok * 4, &sc_full[sc]);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&sc_full[sc], np * kPageTok * 4);
+          for (int p = 0; p < np; ++p)
+            bulk_load(smem + S::OFF_SC + (sc * kTileTok + p * kPageTok) * 4, scales + (int64_t)page[p] * kPageTok,
+                      kPageTok * 4, &sc_full[sc]);
+        }
         ++nsc;
         for (int k = 0; k < NSLAB; ++k, ++it) {
-          const int slot = it % NS;
-          if (it >= NS && !mbar_wait(&empty[slot], (uint32_t)(it / NS - 1) & 1u, abort)) {
+          const int slot = at_slab.slot;
+          if (it >= NS && !__all_sync(0xffffffffu, mbar_wait(&empty[slot], at_slab.phase ^ 1u, abort))) {
             ok = false;
             break;
           }
+          at_slab.step(1);
           uint8_t* dst = smem + S::OFF_RING + slot * S::SLAB;
           const int row = k == 0 ? P * 2 : 128;  // bytes of a slab's row
-          mbar_arrive_expect_tx(&full[slot], np * kPageTok * row);
-          for (int p = 0; p < np; ++p) {
-            if (k == 0) tma_load_2d(dst + p * kPageTok * row, &map_rope, &full[slot], R, page[p] * kPageTok, policy);
-            else tma_load_2d(dst + p * kPageTok * row, &map_lat, &full[slot], (k - 1) * 128, page[p] * kPageTok, policy);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&full[slot], np * kPageTok * row);
+            for (int p = 0; p < np; ++p)
+              tma_load_2d(dst + p * kPageTok * row, k == 0 ? &map_rope : &map_lat, &full[slot],
+                          k == 0 ? R : (k - 1) * 128, page[p] * kPageTok, policy);
           }
         }
       }
@@ -347,7 +385,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------- MMA issuer
-    if (lane == 0 && count > 0) {
+    // The whole warp walks and waits; one elected lane issues.  (Issued from a
+    // lane == 0 branch an MMA costs 147 cycles whatever its N, measured;
+    // elected, with operands in uniform registers, 42 at N = 32, 50 at 64, 66
+    // at 128: the operands' shared-memory reads.)
+    if (count > 0) {
       constexpr uint32_t kMN = (1u << 15) | (1u << 16);  // A and B MN-major
       constexpr uint32_t ID_QK = idesc_e4m3_f32(128, 2 * HB), ID_QR = idesc_bf16_f32(128, HB, 0, 0);
       constexpr uint32_t ID_PV = idesc_e4m3_f32(128, HB) | kMN;
@@ -360,110 +402,138 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t d_p = smem_desc(smem_base + S::OFF_P, 128, kTileTok * 16, kSwizzleNone);
       const uint64_t d_slab = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
       const uint64_t d_rope = P == 64 ? d_slab : smem_desc(smem_base + S::OFF_RING, 16, 512, kSwizzle64B);
-      auto slot_of = [&](int64_t n, int k) { return (int)((n * NSLAB + k) % NS); };
-      auto parity_of = [&](int64_t n, int k) { return (uint32_t)((n * NSLAB + k) / NS) & 1u; };
+      Cursor<NS> here, ahead;  // first slab of tile n, and of the tile QK is at
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+      };
       bool ok = true;
       // step 0: latents 0; step 1: rope; steps 2 ..: latents 1 ..
-      auto qk_step = [&](int64_t n, int step) {
+      auto qk_step = [&](uint32_t buf, int step) {
         const int k = step == 0 ? 1 : step == 1 ? 0 : step;  // slab of the tile, in load order
-        const int slot = slot_of(n, k);
-        if (!mbar_wait(&full[slot], parity_of(n, k), abort)) return false;
+        const Cursor<NS> c = ahead.plus(k);
+        const int slot = c.slot;
+        if (!wait(&full[slot], c.phase)) return false;
         tc_fence_after();
-        const uint32_t d = tmem + S::T_S + (uint32_t)(n & 1) * 2 * HB;
-        const uint64_t off = (uint64_t)(slot * S::SLAB) >> 4;
-        if (k == 0) {
+        const uint32_t d = tmem + S::T_S + buf * 2 * HB;
+        const uint32_t off = (uint32_t)(slot * S::SLAB) >> 4;
+        if (elect_one()) {
+          if (k == 0) {
 #pragma unroll
-          for (int ks = 0; ks < P / 16; ++ks) mma_bf16_ss(d, d_rope + off + ks * 2, d_qr + ks * 2, ID_QR, 1u);
-          tc_commit(&empty[slot]);
-        } else {
-          const uint64_t qoff = (uint64_t)((k - 1) * 2 * HB * 128) >> 4;
+            for (int ks = 0; ks < P / 16; ++ks) mma_bf16_ss(d, d_rope + off + ks * 2, d_qr + ks * 2, ID_QR, 1u);
+            tc_commit(&empty[slot]);
+          } else {
+            const uint32_t qoff = (uint32_t)((k - 1) * 2 * HB * 128) >> 4;
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            mma_f8_ss(d, d_slab + off + ks * 2, d_q8 + qoff + ks * 2, ID_QK, k > 1 || ks > 0 ? 1u : 0u);
+            for (int ks = 0; ks < 4; ++ks)
+              mma_f8_ss(d, d_slab + off + ks * 2, d_q8 + qoff + ks * 2, ID_QK, k > 1 || ks > 0 ? 1u : 0u);
+          }
         }
         return true;
       };
-      int seg = 0;  // segments begun
-      ok = mbar_wait(q_ready, 0, abort);
-      ++seg;
-      for (int s = 0; ok && s < NSLAB; ++s) ok = qk_step(0, s);
-      if (ok) tc_commit(&s_full[0]);
-      for (int64_t n = 0; ok && n < count; ++n) {
+      int seg = 0;  // segments whose query was waited for
+      bool first = true;  // tile n begins a segment
+      // n = -1: tile 0's QK alone
+#pragma unroll 1
+      for (int n = -1; ok && n < count; ++n) {
         const bool more = n + 1 < count;
-        bool fresh = false;  // tile n + 1 begins a sequence
-        if (more) {
-          w.next();
-          fresh = w.tile == 0;
+        if (n >= 0) {
+          here = ahead;
+          ahead.step(NSLAB);
+          if (more) w.next();
         }
-        int s = 0;
-        if (more && !fresh)
-          for (; ok && s < S::LA; ++s) ok = qk_step(n + 1, s);
-        if (ok && more && !fresh && S::LA == NSLAB) tc_commit(&s_full[(n + 1) & 1]);
-        if (!ok || !mbar_wait(p_full, (uint32_t)n & 1u, abort)) { ok = false; break; }
-        if (n > 0 && !mbar_wait(o_free, (uint32_t)(n - 1) & 1u, abort)) { ok = false; break; }
-        tc_fence_after();
-        for (int g = 0; g < NL; ++g) {
-          const int slot = slot_of(n, 1 + g);
-          const uint64_t a = d_slab + ((uint64_t)(slot * S::SLAB) >> 4);
-          const uint32_t d = tmem + S::T_O + g * HB;
+        const bool fresh = more && (n < 0 || w.tile == 0);  // tile n + 1 begins a segment
+        const int early = !more || fresh ? 0 : S::LA;       // its QK steps before tile n's PV
+#pragma unroll 1
+        for (int half = 0; ok && half < 2; ++half) {
+          if (half == 1) {
+            if (n >= 0) {
+              ok = wait(p_full, (uint32_t)n & 1u);
+              if (ok && first && seg > 1) ok = wait(o_free, (uint32_t)(seg - 2) & 1u);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll 1
+              for (int g = 0; g < NL; ++g) {
+                const int slot = here.plus(1 + g).slot;
+                const uint64_t a = d_slab + ((uint32_t)(slot * S::SLAB) >> 4);
+                const uint32_t d = tmem + S::T_O + g * HB;
+                if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kTileTok / 32; ++ks) {
-            mma_f8_ss(d, a + ks * (4096 >> 4), d_p + ks * (512 >> 4), ID_PV, ks > 0 ? 1u : 0u);
-            mma_f8_ss(d, a + ks * (4096 >> 4), d_p + (S::P_BYTES >> 4) + ks * (512 >> 4), ID_PV, 1u);
+                  for (int ks = 0; ks < kTileTok / 32; ++ks) {
+                    mma_f8_ss(d, a + ks * (4096 >> 4), d_p + ks * (512 >> 4), ID_PV, first && ks == 0 ? 0u : 1u);
+                    mma_f8_ss(d, a + ks * (4096 >> 4), d_p + (S::P_BYTES >> 4) + ks * (512 >> 4), ID_PV, 1u);
+                  }
+                  tc_commit(&empty[slot]);
+                }
+              }
+              commit(pv_done);
+            }
+            first = fresh;
+            if (fresh) {
+              ok = wait(q_ready, (uint32_t)seg & 1u);
+              ++seg;
+            }
           }
-          tc_commit(&o_full[g]);
-          tc_commit(&empty[slot]);
-        }
-        if (more && (fresh || S::LA < NSLAB)) {
-          if (fresh) {
-            if (!mbar_wait(q_ready, (uint32_t)seg & 1u, abort)) { ok = false; break; }
-            ++seg;
+#pragma unroll 1
+          for (int st = half == 0 ? 0 : early; ok && st < (half == 0 ? early : more ? NSLAB : 0); ++st) {
+            ok = qk_step((uint32_t)(n + 1) & 1u, st);
+            if (ok && st == NSLAB - 1) commit(&s_full[(n + 1) & 1]);
           }
-          for (; ok && s < NSLAB; ++s) ok = qk_step(n + 1, s);
-          if (ok) tc_commit(&s_full[(n + 1) & 1]);
         }
       }
       if (!ok) raise_abort(abort, status, kStatusTimeout);
       // every issued MMA must finish before TMEM and shared memory are released
-      tc_commit(drain);
+      commit(drain);
       mbar_wait(drain, 0, no_abort);
     }
-  } else if (count > 0) {
+  } else {
     // ------------------------------------------- softmax / accumulate warps
+    if (count > 0) {
     const int wg = warp >> 2, quarter = warp & 3;
     const int j = quarter * 32 + lane;  // token of the tile; row of an O^T block
     const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
     float* red = reinterpret_cast<float*>(smem + S::OFF_RED);
     float* lred = reinterpret_cast<float*>(smem + S::OFF_LRED);
-    float* ab = reinterpret_cast<float*>(smem + S::OFF_AB) + warp * 2 * HW;
     float* mt = reinterpret_cast<float*>(smem + S::OFF_MT) + warp * HW;
     float* fh = reinterpret_cast<float*>(smem + S::OFF_FH);
     const int h0 = hg * HB;  // first head of the group
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
 
     // Query digits of sequence b: a warp per head, 16 (4) latents a lane.  A
     // warpgroup loads its own heads: its warps have all read the old factors
     // (fh) when one of them is past the tile's rendezvous.
     auto load_q = [&](int b) {
-      constexpr int CPL = R / 32;  // latents per lane
+      constexpr int CPL = R / 32;               // latents per lane
+      constexpr int NQ = HW / 4 < 4 ? HW / 4 : 4;  // heads whose loads are in flight together
 #pragma unroll 1
-      for (int h = wg * HW + quarter; h < (wg + 1) * HW; h += 4) {
-        const bool live = h0 + h < H;
-        const int64_t row = (int64_t)b * H + h0 + h;
-        uint32_t x[CPL / 2];
-        uint4 r = make_uint4(0, 0, 0, 0);
+      for (int i0 = 0; i0 < HW / 4; i0 += NQ) {
+      uint32_t xs[NQ][CPL / 2];
+      uint4 rs[NQ];
 #pragma unroll
-        for (int i = 0; i < CPL / 2; ++i) x[i] = 0;
-        if (live) {
+      for (int q = 0; q < NQ; ++q) {
+        const int h = wg * HW + quarter + 4 * (i0 + q);
+        const int64_t row = (int64_t)b * H + h0 + h;
+        rs[q] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < CPL / 2; ++i) xs[q][i] = 0;
+        if (h0 + h < H) {
           if constexpr (CPL == 16) {
             const uint4* src = reinterpret_cast<const uint4*>(q_lat + row * R + lane * 16);
             const uint4 u = src[0], v = src[1];
-            x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+            xs[q][0] = u.x, xs[q][1] = u.y, xs[q][2] = u.z, xs[q][3] = u.w;
+            xs[q][4] = v.x, xs[q][5] = v.y, xs[q][6] = v.z, xs[q][7] = v.w;
           } else {
             const uint2 u = *reinterpret_cast<const uint2*>(q_lat + row * R + lane * 4);
-            x[0] = u.x, x[1] = u.y;
+            xs[q][0] = u.x, xs[q][1] = u.y;
           }
-          if (lane < P / 8) r = *reinterpret_cast<const uint4*>(q_rope + row * P + lane * 8);
+          if (lane < P / 8) rs[q] = *reinterpret_cast<const uint4*>(q_rope + row * P + lane * 8);
         }
+      }
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) {
+        const int h = wg * HW + quarter + 4 * (i0 + q);
+        const uint32_t (&x)[CPL / 2] = xs[q];
+        const uint4 r = rs[q];
         const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
         float am = 0.0f, rm = 0.0f;
 #pragma unroll
@@ -504,213 +574,242 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (lane == 0) fh[h] = exp2i(e) * scale_log2;
       }
+      }
       fence_proxy_async_shared();
       warp_arrive(q_ready);
     };
 
-    float acc[NL][HW];
-    float m_run = -INFINITY, l_run = 0.0f;  // of head lane % HW, the sum over this warp's tokens
-#pragma unroll
-    for (int g = 0; g < NL; ++g)
-#pragma unroll
-      for (int h = 0; h < HW; ++h) acc[g][h] = 0.0f;
+    // Probabilities and sums are in units of 2^r, r a per-head reference (held
+    // by lane head % HW) that stays within kRefLow .. kRefHigh above each
+    // tile's maximum: a probability then keeps its digits whatever came
+    // before it.  When a tile's maximum leaves that window, the reference
+    // moves (kRefNew above it) and the head's columns of O^T are rescaled in
+    // TMEM; fp32 has the range for both directions (r never falls more than
+    // 2^40 below the largest: what far is out of an fp32 sum's reach).
+    constexpr float kRefNew = 4.0f, kRefHigh = 8.0f, kRefLow = -0.8f;
+    float ls[HW];  // softmax sums over this thread's tokens
+    float r_ref = 0.0f, r_top = 0.0f;
     int meet = 0;  // phase of wg_bar
-    bool ok = true;
-    bool shared_front = w.tile != 0;  // the segment's sequence began in an earlier run
-    int n_seg = 0;
-    load_q(w.b);
-    for (int64_t n = 0; n < count; ++n) {
-      const int valid = w.valid();
+    bool ok = true, first = true;       // first: the tile begins a segment
+    bool shared_front = w.tile != 0;    // the segment's sequence began in an earlier run
+    int n_seg = 0, sc = 0;
+    uint32_t sc_phase = 0;
+    // n = -1: the first query alone
+#pragma unroll 1
+    for (int n = -1; n < count; ++n) {
       const int b_now = w.b;
-      const bool seq_end = w.tile == w.ntile - 1;
+      const bool seq_end = n < 0 || w.tile == w.ntile - 1;
       const bool seg_end = seq_end || n + 1 == count;
-      const int sc = (int)(n % kScaleStages);
-      if (!__all_sync(0xffffffffu, mbar_wait(&sc_full[sc], (uint32_t)(n / kScaleStages) & 1u, abort))) { ok = false; break; }
-      // a scale of zero (a row never written) counts as a tiny one
-      const float sigma = j < valid ? fmaxf(reinterpret_cast<const float*>(smem + S::OFF_SC)[sc * kTileTok + j], 0x1p-100f)
-                                    : 1.0f;
-      warp_arrive(&sc_empty[sc]);
-      const float lsig = __log2f(sigma), isig = __frcp_rn(sigma);
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[n & 1], (uint32_t)(n >> 1) & 1u, abort))) { ok = false; break; }
-      tc_fence_after();
-      float u[HW];
-      {
-        float lo[HW];
-        const uint32_t ts = t_lane + S::T_S + (uint32_t)(n & 1) * 2 * HB + wg * HW;
-        tmem_ld(ts, u);
-        tmem_ld(ts + HB, lo);
+      if (n >= 0) {
+        const int valid = w.valid();
+        if (!wait(&sc_full[sc], sc_phase)) { ok = false; break; }
+        // a scale of zero (a row never written) counts as a tiny one
+        const float sigma =
+            j < valid ? fmaxf(reinterpret_cast<const float*>(smem + S::OFF_SC)[sc * kTileTok + j], 0x1p-100f) : 1.0f;
+        warp_arrive(&sc_empty[sc]);
+        if (++sc == kScaleStages) {
+          sc = 0;
+          sc_phase ^= 1u;
+        }
+        const float lsig = __log2f(sigma), isig = __frcp_rn(sigma);
+        if (!wait(&s_full[n & 1], (uint32_t)(n >> 1) & 1u)) { ok = false; break; }
+        tc_fence_after();
+        float u[HW];
+        {
+          constexpr int HC = HW < 16 ? HW : 16;  // heads read at once
+          const uint32_t ts = t_lane + S::T_S + (uint32_t)(n & 1) * 2 * HB + wg * HW;
+#pragma unroll
+          for (int c = 0; c < HW; c += HC) {
+            uint32_t s_hi[HC], s_lo[HC];
+            tmem_ld(ts + c, s_hi);
+            tmem_ld(ts + HB + c, s_lo);
+            tmem_ld_wait();
+            auto score = [&](int h, float f) {
+              u[c + h] = fmaf((__uint_as_float(s_hi[h]) + __uint_as_float(s_lo[h])) * sigma, f, lsig);
+            };
+#pragma unroll
+            for (int h = 0; h < HC; h += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(fh + wg * HW + c + h);
+              score(h, f.x);
+              score(h + 1, f.y);
+              score(h + 2, f.z);
+              score(h + 3, f.w);
+            }
+          }
+          if (valid < kTileTok && j >= valid) {
+#pragma unroll
+            for (int h = 0; h < HW; ++h) u[h] = -INFINITY;
+          }
+        }
+        // the tile's maximum per head: over the warp's tokens, then the warpgroup's
+        float mine = 0.0f;
+#pragma unroll
+        for (int h = 0; h < HW; ++h) {
+          const float r = redux_max(u[h]);
+          if (lane % HW == h) mine = r;
+        }
+        float* red_n = red + ((n & 1) * NWG + wg) * 4 * HW;
+        if (lane < HW) red_n[quarter * HW + lane] = mine;
+        warp_arrive(&wg_bar[wg]);
+        if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
+        ++meet;
+        const int hl = lane % HW;
+        float t = fmaxf(fmaxf(red_n[hl], red_n[HW + hl]), fmaxf(red_n[2 * HW + hl], red_n[3 * HW + hl]));
+        if (t == -INFINITY) t = 0.0f;
+        r_top = first ? t : fmaxf(r_top, t);
+        const float want = fmaxf(t, r_top - 40.0f);
+        const bool move = first || !(r_ref >= want + kRefLow && r_ref <= want + kRefHigh);
+        // the previous PV has read P and written O^T
+        if (n > 0 && !wait(pv_done, (uint32_t)(n - 1) & 1u)) { ok = false; break; }
+        if (uint32_t moved = __ballot_sync(0xffffffffu, move)) {
+          const float to = want + kRefNew;
+          const float f = !move ? 1.0f : fast_exp2(r_ref - to);
+          if (move) r_ref = to;
+          if (first) {
+#pragma unroll
+            for (int h = 0; h < HW; ++h) ls[h] = 0.0f;
+          } else {
+#pragma unroll
+            for (int h = 0; h < HW; ++h) ls[h] *= __shfl_sync(0xffffffffu, f, h);
+            tc_fence_after();
+            moved &= 0xffffffffu >> (32 - HW);
+#pragma unroll 1
+            while (moved != 0) {
+              const int h = __ffs(moved) - 1;
+              moved &= moved - 1;
+              const float fh1 = __shfl_sync(0xffffffffu, f, h);
+              uint32_t o[NL];
+#pragma unroll
+              for (int g = 0; g < NL; ++g) tmem_ld1(t_lane + S::T_O + g * HB + wg * HW + h, o[g]);
+              tmem_ld_wait();
+#pragma unroll
+              for (int g = 0; g < NL; ++g)
+                tmem_st1(t_lane + S::T_O + g * HB + wg * HW + h, __float_as_uint(__uint_as_float(o[g]) * fh1));
+            }
+            tmem_st_wait();
+          }
+          if (lane < HW) mt[lane] = r_ref - 8.0f;
+          __syncwarp();
+        }
+        // probabilities in units of 2^(r - 8), their sums and digits
+        uint32_t hi[HW / 4], lo[HW / 4];
 #pragma unroll
         for (int h = 0; h < HW; h += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(fh + wg * HW + h);
-          u[h + 0] = fmaf((u[h + 0] + lo[h + 0]) * sigma, f.x, lsig);
-          u[h + 1] = fmaf((u[h + 1] + lo[h + 1]) * sigma, f.y, lsig);
-          u[h + 2] = fmaf((u[h + 2] + lo[h + 2]) * sigma, f.z, lsig);
-          u[h + 3] = fmaf((u[h + 3] + lo[h + 3]) * sigma, f.w, lsig);
+          const float4 r = *reinterpret_cast<const float4*>(mt + h);
+          u[h + 0] = fast_exp2(u[h + 0] - r.x);
+          u[h + 1] = fast_exp2(u[h + 1] - r.y);
+          u[h + 2] = fast_exp2(u[h + 2] - r.z);
+          u[h + 3] = fast_exp2(u[h + 3] - r.w);
+          ls[h + 0] = fmaf(u[h + 0], isig, ls[h + 0]);
+          ls[h + 1] = fmaf(u[h + 1], isig, ls[h + 1]);
+          ls[h + 2] = fmaf(u[h + 2], isig, ls[h + 2]);
+          ls[h + 3] = fmaf(u[h + 3], isig, ls[h + 3]);
+          uint32_t a, b2, c, d;
+          split_digits(u[h + 0], u[h + 1], a, b2);
+          split_digits(u[h + 2], u[h + 3], c, d);
+          hi[h / 4] = a | (c << 16);
+          lo[h / 4] = b2 | (d << 16);
         }
-        if (valid < kTileTok) {
+        {
+          uint8_t* dst = smem + S::OFF_P + (wg * HW / 16) * (kTileTok * 16) + j * 16 + (wg * HW) % 16;
+          if constexpr (HW >= 16) {
 #pragma unroll
-          for (int h = 0; h < HW; ++h) u[h] = j < valid ? u[h] : -INFINITY;
-        }
-      }
-      // the tile's maximum per head: over the warp's tokens, then the warpgroup's
-      float mine = 0.0f;
-#pragma unroll
-      for (int h = 0; h < HW; ++h) {
-        const float r = redux_max(u[h]);
-        if (lane % HW == h) mine = r;
-      }
-      float* red_n = red + (((int)(n & 1) * 2 + wg) * 4) * HW;
-      if (lane < HW) red_n[quarter * HW + lane] = mine;
-      if (!__all_sync(0xffffffffu, mbar_rendezvous(&wg_bar[wg], meet, abort))) { ok = false; break; }
-      {
-        const int h = lane % HW;
-        float t = fmaxf(fmaxf(red_n[h], red_n[HW + h]), fmaxf(red_n[2 * HW + h], red_n[3 * HW + h]));
-        if (t == -INFINITY) t = 0.0f;
-        const float top = fmaxf(m_run, t);
-        const float a = fast_exp2(m_run - top), bt = fast_exp2(t - top);
-        m_run = top;
-        l_run *= a;
-        if (lane < HW) {
-          mt[lane] = t;
-          ab[lane] = a;
-          ab[HW + lane] = bt;
-        }
-        __syncwarp();
-        mine = bt;
-      }
-      // probabilities in units of 2^-8 of the tile's largest, their sum and digits
-      uint32_t hi[HW / 4], lo[HW / 4];
-#pragma unroll
-      for (int h = 0; h < HW; h += 4) {
-        const float4 t = *reinterpret_cast<const float4*>(mt + h);
-        u[h + 0] = fast_exp2(u[h + 0] - t.x + 8.0f);
-        u[h + 1] = fast_exp2(u[h + 1] - t.y + 8.0f);
-        u[h + 2] = fast_exp2(u[h + 2] - t.z + 8.0f);
-        u[h + 3] = fast_exp2(u[h + 3] - t.w + 8.0f);
-        uint32_t a, b2, c, d;
-        split_digits(u[h + 0], u[h + 1], a, b2);
-        split_digits(u[h + 2], u[h + 3], c, d);
-        hi[h / 4] = a | (c << 16);
-        lo[h / 4] = b2 | (d << 16);
-      }
-      {
-        uint8_t* dst = smem + S::OFF_P + (wg * HW / 16) * (kTileTok * 16) + j * 16 + (wg * HW) % 16;
-        if constexpr (HW >= 16) {
-#pragma unroll
-          for (int i = 0; i < HW / 16; ++i) {
-            *reinterpret_cast<uint4*>(dst + i * (kTileTok * 16)) =
-                make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-            *reinterpret_cast<uint4*>(dst + S::P_BYTES + i * (kTileTok * 16)) =
-                make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+            for (int i = 0; i < HW / 16; ++i) {
+              *reinterpret_cast<uint4*>(dst + i * (kTileTok * 16)) =
+                  make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
+              *reinterpret_cast<uint4*>(dst + S::P_BYTES + i * (kTileTok * 16)) =
+                  make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+            }
+          } else {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(dst + S::P_BYTES) = make_uint2(lo[0], lo[1]);
           }
-        } else {
-          *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-          *reinterpret_cast<uint2*>(dst + S::P_BYTES) = make_uint2(lo[0], lo[1]);
         }
-      }
-      if (j >= valid) {
-        // whatever lies past the sequence's end must not meet a zero
-        // probability as NaN: this warpgroup clears its half of the slabs
-        const uint4 z = make_uint4(0, 0, 0, 0);
-        for (int g = wg; g < NL; g += 2) {
-          uint4* r = reinterpret_cast<uint4*>(smem + S::OFF_RING + (int)((n * NSLAB + 1 + g) % NS) * S::SLAB + j * 128);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) r[i] = z;
+        if (j >= valid) {
+          // whatever lies past the sequence's end must not meet a zero
+          // probability as NaN: this warpgroup clears its share of the slabs
+          const uint4 z = make_uint4(0, 0, 0, 0);
+          for (int g = wg; g < NL; g += NWG) {
+            uint4* r = reinterpret_cast<uint4*>(smem + S::OFF_RING + (int)(((int64_t)n * NSLAB + 1 + g) % NS) * S::SLAB + j * 128);
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) r[i] = z;
+          }
         }
+        fence_proxy_async_shared();
+        tc_fence_before();
+        warp_arrive(p_full);
+        first = false;
+        if (n + 1 < count) w.next();
       }
-      fence_proxy_async_shared();
-      warp_arrive(p_full);
-      // softmax sum: each lane ends with head lane % HW over the warp's tokens
-#pragma unroll
-      for (int h = 0; h < HW; ++h) u[h] *= isig;
+      if (!seg_end) continue;
+      if (n + 1 < count) load_q(w.b);  // the old query's last QK is done
+      if (n < 0) continue;
+
+      // ------------------------------------------------ the segment's result
+      // softmax sums over the warp's tokens (lane head % HW), then the warpgroup's
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) {
         if (o >= HW) {
 #pragma unroll
-          for (int h = 0; h < HW; ++h) u[h] += __shfl_xor_sync(0xffffffffu, u[h], o);
+          for (int h = 0; h < HW; ++h) ls[h] += __shfl_xor_sync(0xffffffffu, ls[h], o);
         } else {
           const bool up = (lane & o) != 0;
 #pragma unroll
           for (int h = 0; h < o; ++h) {
-            const float give = up ? u[h] : u[h + o], keep = up ? u[h + o] : u[h];
-            u[h] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            const float give = up ? ls[h] : ls[h + o], keep = up ? ls[h + o] : ls[h];
+            ls[h] = keep + __shfl_xor_sync(0xffffffffu, give, o);
           }
         }
       }
-      l_run = fmaf(u[0], mine, l_run);
-      if (n + 1 < count) {
-        w.next();
-        if (seg_end) load_q(w.b);  // the old query's last QK is done
-      }
-      // this tile's O^T into the registers, block by block as it is finished
-      bool good = true;
-#pragma unroll
-      for (int g = 0; g < NL; ++g) {
-        good = good && __all_sync(0xffffffffu, mbar_wait(&o_full[g], (uint32_t)n & 1u, abort));
-        if (!good) break;
-        tc_fence_after();
-        float o[HW];
-        tmem_ld(t_lane + S::T_O + g * HB + wg * HW, o);
-#pragma unroll
-        for (int h = 0; h < HW; h += 4) {
-          const float4 a = *reinterpret_cast<const float4*>(ab + h), bt = *reinterpret_cast<const float4*>(ab + HW + h);
-          acc[g][h + 0] = fmaf(acc[g][h + 0], a.x, o[h + 0] * bt.x);
-          acc[g][h + 1] = fmaf(acc[g][h + 1], a.y, o[h + 1] * bt.y);
-          acc[g][h + 2] = fmaf(acc[g][h + 2], a.z, o[h + 2] * bt.z);
-          acc[g][h + 3] = fmaf(acc[g][h + 3], a.w, o[h + 3] * bt.w);
-        }
-      }
-      if (!good) { ok = false; break; }
-      tc_fence_before();
-      warp_arrive(o_free);
-      if (!seg_end) continue;
-
-      // ------------------------------------------------ the segment's result
-      if (lane < HW) lred[(wg * 4 + quarter) * HW + lane] = l_run;
-      if (!__all_sync(0xffffffffu, mbar_rendezvous(&wg_bar[wg], meet, abort))) { ok = false; break; }
+      if (lane < HW) lred[(wg * 4 + quarter) * HW + lane] = ls[0];
+      warp_arrive(&wg_bar[wg]);
+      if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
+      ++meet;
       const int hl = lane % HW;
       const float l = lred[(wg * 4 + 0) * HW + hl] + lred[(wg * 4 + 1) * HW + hl] + lred[(wg * 4 + 2) * HW + hl] +
                       lred[(wg * 4 + 3) * HW + hl];
       const int hb = h0 + wg * HW;  // first head of this warpgroup
-      if (!shared_front && seq_end) {
-        if (lane < HW) mt[lane] = 1.0f / l;
-        __syncwarp();
-        const bool odd = lane & 1;
-#pragma unroll
-        for (int h = 0; h < HW; h += 2) {
-          const float2 il = *reinterpret_cast<const float2*>(mt + h);
-          const int head = hb + h + (odd ? 1 : 0);
-          // lanes swap so that each stores two columns of one head
-          __nv_bfloat16* dst = out + ((int64_t)b_now * H + head) * R + quarter * 32 + (lane & ~1);
-#pragma unroll
-          for (int g = 0; g < NL; ++g) {
-            const float x = acc[g][h] * il.x, y = acc[g][h + 1] * il.y;
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? x : y, 1);
-            if (head < H) *reinterpret_cast<uint32_t*>(dst + g * 128) = odd ? pack_bf16x2(got, y) : pack_bf16x2(x, got);
-          }
-        }
-        __syncwarp();
-      } else {
-        const int64_t slot = (int64_t)blockIdx.x * 2 + (n_seg > 0 ? 1 : 0);
-        float* dst = ws_o + (slot * HB + wg * HW) * R + j;
-#pragma unroll
-        for (int h = 0; h < HW; ++h)
-          if (hb + h < H) {
-#pragma unroll
-            for (int g = 0; g < NL; ++g) dst[(int64_t)h * R + g * 128] = acc[g][h];
-          }
-        if (quarter == 0 && lane < HW) ws_ml[slot * HB + wg * HW + lane] = make_float2(m_run, l);
+      const bool whole = !shared_front && seq_end;
+      const int64_t slot = (int64_t)blockIdx.x * 2 + (n_seg > 0 ? 1 : 0);
+      if (lane < HW) {
+        mt[lane] = 1.0f / l;
+        if (!whole && quarter == 0) ws_ml[slot * HB + wg * HW + lane] = make_float2(r_ref, l);
       }
+      __syncwarp();
+      if (!wait(pv_done, (uint32_t)n & 1u)) { ok = false; break; }
+      tc_fence_after();
+      const bool odd = lane & 1;
+#pragma unroll 1
+      for (int g = 0; g < NL; ++g) {
+        uint32_t o[HW];
+        tmem_ld(t_lane + S::T_O + g * HB + wg * HW, o);
+        tmem_ld_wait();
+        if (whole) {
+          // lanes swap so that each stores two columns of one head
+          __nv_bfloat16* dst = out + ((int64_t)b_now * H + hb + (odd ? 1 : 0)) * R + g * 128 + quarter * 32 + (lane & ~1);
 #pragma unroll
-      for (int g = 0; g < NL; ++g)
+          for (int h = 0; h < HW; h += 2) {
+            const float2 il = *reinterpret_cast<const float2*>(mt + h);
+            const float x = __uint_as_float(o[h]) * il.x, y = __uint_as_float(o[h + 1]) * il.y;
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? x : y, 1);
+            if (hb + h + (odd ? 1 : 0) < H)
+              *reinterpret_cast<uint32_t*>(dst + h * R) = odd ? pack_bf16x2(got, y) : pack_bf16x2(x, got);
+          }
+        } else {
+          float* dst = ws_o + (slot * HB + wg * HW) * R + g * 128 + j;
 #pragma unroll
-        for (int h = 0; h < HW; ++h) acc[g][h] = 0.0f;
-      m_run = -INFINITY;
-      l_run = 0.0f;
+          for (int h = 0; h < HW; ++h)
+            if (hb + h < H) dst[h * R] = __uint_as_float(o[h]);
+        }
+      }
+      tc_fence_before();
+      warp_arrive(o_free);
+      first = true;
       shared_front = false;
       ++n_seg;
     }
     if (!ok) raise_abort(abort, status, kStatusTimeout);
+    }
   }
 
   tc_fence_before();
@@ -751,7 +850,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
   const int64_t cta0 = (int64_t)(h / HB) * runs, hl = h % HB;
   // the first run's segment of this sequence is its last one: its second
   // slot, unless the run also begins there
-  auto slot_of = [&](int i) { return (cta0 + i) * 2 + (i == i0 && run_start(i, T, runs) != t0 ? 1 : 0); };
+  const int second = run_start(i0, T, runs) != t0 ? 1 : 0;
+  const bool gaps = T < runs;
   float m = -INFINITY, l = 0.0f;
   float4 o[V];
 #pragma unroll
@@ -761,10 +861,10 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
   for (int i = i0 + (kWarpPerHead ? 0 : warp); i <= i1; i += kStep) {
     // a run between i0 and i1 may be empty only when there are fewer tiles
     // than runs; it then wrote nothing
-    if (run_start(i, T, runs) == run_start(i + 1, T, runs)) continue;
-    const int64_t s = slot_of(i) * HB + hl;
+    if (gaps && run_start(i, T, runs) == run_start(i + 1, T, runs)) continue;
+    const int64_t s = ((cta0 + i) * 2 + (i == i0 ? second : 0)) * HB + hl;
     const float2 ml = ws_ml[s];
-    const float mn = fmaxf(m, ml.x), a = exp2f(m - mn), c = exp2f(ml.x - mn);
+    const float mn = fmaxf(m, ml.x), a = fast_exp2(m - mn), c = fast_exp2(ml.x - mn);
     m = mn;
     l = l * a + ml.y * c;
 #pragma unroll
@@ -792,7 +892,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
     for (int i = 0; i < kCombineWarps; ++i) top = fmaxf(top, sm[i]);
     for (int i = 0; i < kCombineWarps; ++i) {
       if (sm[i] == -INFINITY) continue;  // no partial
-      const float c = exp2f(sm[i] - top);
+      const float c = fast_exp2(sm[i] - top);
       const float4 x = so[i][warp * 32 + lane];
       den += sl[i] * c;
       r.x += x.x * c;
@@ -841,7 +941,7 @@ int launch(dsb_ctx* ctx, const void* q_lat, const void* q_rope, const void* cach
   auto kern = decode_fp8_kernel<R, P, HB>;
   static std::atomic<bool> attr_set[kMaxDevices];
   if (rc = smem_attr_once(ctx, kern, S::SMEM_BYTES, attr_set); rc != DSB_OK) return rc;
-  DSB_CUDA_TRY(ctx, launch_pdl(kern, dim3((unsigned)(groups * runs)), kThreads, S::SMEM_BYTES, ctx->stream, map_lat,
+  DSB_CUDA_TRY(ctx, launch_pdl(kern, dim3((unsigned)(groups * runs)), S::THREADS, S::SMEM_BYTES, ctx->stream, map_lat,
                                map_rope, static_cast<const __nv_bfloat16*>(q_lat),
                                static_cast<const __nv_bfloat16*>(q_rope), scales, n_blocks, block_table, max_blocks,
                                seq_lens, B, H, runs, softmax_scale * 1.4426950408889634f,
