@@ -59,16 +59,14 @@ template <int R, int P, int HB>
 struct Shape {
   static constexpr int NL = R / 128;                 // latent slabs per tile
   static constexpr int NSLAB = NL + 1;               // + rope
-  static constexpr int NWG = HB == 64 ? 4 : 2;       // softmax warpgroups
+  static constexpr int NWG = 2;                      // softmax warpgroups
   static constexpr int SM_WARPS = NWG * 4;
-  static constexpr int THREADS = (SM_WARPS + 2) * 32;  // + TMA and MMA
+  static constexpr int THREADS = (SM_WARPS + 3) * 32;  // + TMA, QK and PV
   static constexpr int HW = HB / NWG;                // heads per warpgroup
   static constexpr int SLAB = kTileTok * 128;        // bytes
   static constexpr int NS = HB == 16 ? 12 : HB == 32 || NL == 1 ? 10 : 8;  // ring slots: what fits
-  // slabs of tile n + 1's QK issued before tile n's PV: all when two tiles
-  // fit, else as many as the ring can hold beside tile n's latents
-  static constexpr int LA = NS >= 2 * NSLAB ? NSLAB : NS - NL;
-  static_assert(LA >= 1 && LA <= NSLAB, "ring");
+  static_assert(NS >= NSLAB + 1, "ring");
+  static constexpr bool PREFETCH = NS < 2 * NSLAB;
   static constexpr int Q8_BYTES = 2 * HB * R;        // [slab][hi heads | lo heads][128 B], SW128
   static constexpr int QR_BYTES = HB * P * 2;        // [head][P bf16], SW128 (P = 64) or SW64
   static constexpr int P_BYTES = HB * kTileTok;      // one digit of the probabilities
@@ -81,7 +79,7 @@ struct Shape {
   static constexpr int OFF_LRED = OFF_RED + 2 * 4 * HB * 4;              // [NWG][4 warps][HW] sums
   static constexpr int OFF_MT = OFF_LRED + 4 * HB * 4;                   // per warp [HW]: references (or 1 / sums)
   static constexpr int OFF_FH = OFF_MT + 4 * HB * 4;              // [HB] a_h * scale * log2(e)
-  static constexpr int NBAR = 2 * NS + 2 + 5 + NWG + 2 * kScaleStages;
+  static constexpr int NBAR = 2 * NS + 4 + 6 + NWG + 2 * kScaleStages;
   static constexpr int OFF_BAR = (OFF_FH + HB * 4 + 7) / 8 * 8;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;                    // tmem base, abort flags, start, scan
   static constexpr int SMEM_BYTES = OFF_MISC + 128 + 1024;               // + alignment slack
@@ -93,6 +91,42 @@ struct Shape {
   static constexpr uint32_t T_COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
   static_assert(USED <= 512, "TMEM");
 };
+
+// A warp-uniform value that the compiler then knows to be one: MMA operands
+// computed from it stay in uniform registers, and branches on it do not
+// count as divergent (in either case an MMA would cost 3 times as much).
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// Two floats in one register pair: one instruction for both (fma / add / mul .f32x2).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
 __device__ __forceinline__ float redux_max(float v) {
   float r;
@@ -122,6 +156,12 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// Bring a box into L2 ahead of its load.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y)
+               : "memory");
+}
+
 // N columns of this thread's TMEM lane; tmem_ld_wait() before their use.
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
@@ -135,7 +175,7 @@ __device__ __forceinline__ bool bad_len(int len, int max_blocks) {
 }
 
 __device__ __forceinline__ int tiles_of(int len, int max_blocks) {
-  return bad_len(len, max_blocks) ? 0 : (int)(((int64_t)len + kTileTok - 1) / kTileTok);
+  return bad_len(len, max_blocks) ? 0 : len / kTileTok + (len % kTileTok != 0 ? 1 : 0);
 }
 
 // A run of tiles through the sequences; every role walks its own copy.
@@ -212,14 +252,15 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
   uint64_t* full = bars;                     // [NS] slab landed
   uint64_t* empty = full + NS;               // [NS] slab's last MMA done
   uint64_t* s_full = empty + NS;             // [2] scores of a tile ready
-  uint64_t* pv_done = s_full + 2;            // a tile's PV done
+  uint64_t* s_free = s_full + 2;             // [2] scores read
+  uint64_t* pv_done = s_free + 2;            // a tile's PV done
   uint64_t* p_full = pv_done + 1;            // probabilities of a tile written
   uint64_t* o_free = p_full + 1;             // O^T of a segment read
   uint64_t* q_ready = o_free + 1;            // query digits of a segment written
   uint64_t* wg_bar = q_ready + 1;            // [NWG] rendezvous of a warpgroup
   uint64_t* sc_full = wg_bar + NWG;           // [stages] token scales landed
   uint64_t* sc_empty = sc_full + kScaleStages;
-  uint64_t* drain = sc_empty + kScaleStages;  // every MMA issued is done
+  uint64_t* drain = sc_empty + kScaleStages;  // [2] every MMA that a warp issued is done
   uint32_t* misc = reinterpret_cast<uint32_t*>(smem + S::OFF_MISC);
   volatile int* abort = reinterpret_cast<volatile int*>(misc + 1);
   volatile int* no_abort = reinterpret_cast<volatile int*>(misc + 2);  // never raised: for drain waits
@@ -230,20 +271,23 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
   // uniform registers
   const int warp = __shfl_sync(0xffffffffu, (int)warp_id(), 0), lane = (int)lane_id();
   const int hg = blockIdx.x / runs, run = blockIdx.x % runs;  // head group and run
-  constexpr int kTmaWarp = kSmWarps, kMmaWarp = kSmWarps + 1;
+  constexpr int kTmaWarp = kSmWarps, kQkWarp = kSmWarps + 1, kPvWarp = kSmWarps + 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], kSmWarps);
+      mbar_init(&drain[i], 1);
+    }
     for (int i = 0; i < NWG; ++i) mbar_init(&wg_bar[i], 4);
     mbar_init(pv_done, 1);
     mbar_init(p_full, kSmWarps);
     mbar_init(o_free, kSmWarps);
     mbar_init(q_ready, kSmWarps);
-    mbar_init(drain, 1);
     for (int i = 0; i < kScaleStages; ++i) {
       mbar_init(&sc_full[i], 1);
       mbar_init(&sc_empty[i], kSmWarps);
@@ -270,6 +314,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     const int per = (B + kThreads - 1) / kThreads;
     const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
     int mine = 0;
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       const int len = seq_lens[b];
       if (blockIdx.x == 0 && bad_len(len, max_blocks)) atomicCAS(status, 0, kStatusBadInput);
@@ -295,6 +340,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     count = (int)(run_start(run + 1, T, runs) - run0);
     if (count > 0 && run0 >= before && run0 < before + mine) {
       int t = before, b = b0;
+#pragma unroll 1
       for (;; ++b) {
         const int n = tiles_of(seq_lens[b], max_blocks);
         if (run0 < t + n) break;
@@ -305,6 +351,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     }
     if (blockIdx.x == 0) {  // for combine_kernel
       int t = before;
+#pragma unroll 1
       for (int b = b0; b < b1; ++b) {
         prefix[b] = t;
         t += tiles_of(seq_lens[b], max_blocks);
@@ -313,7 +360,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     }
     __syncthreads();
   }
-  const uint32_t tmem = misc[0];
+  const uint32_t tmem = (uint32_t)uniform((int)misc[0]);
   const uint32_t smem_base = smem_u32(smem);
   Walk w;
   if (count > 0) w.start(seq_lens, B, max_blocks, start[0], start[1]);
@@ -359,6 +406,20 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
                       kPageTok * 4, &sc_full[sc]);
         }
         ++nsc;
+        if (S::PREFETCH && at + 2 < 32) {
+          // the ring holds less than two tiles: the tile after next into L2
+          const int p0 = __shfl_sync(0xffffffffu, pages, at + 2), p1 = __shfl_sync(0xffffffffu, pages, at + 3);
+          const int left = w.len - (w.tile + 2) * kTileTok;
+          if (left > 0 && elect_one()) {
+#pragma unroll 1
+            for (int k = 0; k < NSLAB; ++k) {
+              tma_prefetch_2d(k == 0 ? &map_rope : &map_lat, k == 0 ? R : (k - 1) * 128, p0 * kPageTok);
+              if (left > kPageTok)
+                tma_prefetch_2d(k == 0 ? &map_rope : &map_lat, k == 0 ? R : (k - 1) * 128, p1 * kPageTok);
+            }
+          }
+        }
+#pragma unroll 1
         for (int k = 0; k < NSLAB; ++k, ++it) {
           const int slot = at_slab.slot;
           if (it >= NS && !__all_sync(0xffffffffu, mbar_wait(&empty[slot], at_slab.phase ^ 1u, abort))) {
@@ -368,11 +429,12 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           at_slab.step(1);
           uint8_t* dst = smem + S::OFF_RING + slot * S::SLAB;
           const int row = k == 0 ? P * 2 : 128;  // bytes of a slab's row
+          const int x = k == 0 ? R : (k - 1) * 128;
+          const CUtensorMap* map = k == 0 ? &map_rope : &map_lat;
           if (elect_one()) {
             mbar_arrive_expect_tx(&full[slot], np * kPageTok * row);
-            for (int p = 0; p < np; ++p)
-              tma_load_2d(dst + p * kPageTok * row, k == 0 ? &map_rope : &map_lat, &full[slot],
-                          k == 0 ? R : (k - 1) * 128, page[p] * kPageTok, policy);
+            tma_load_2d(dst, map, &full[slot], x, page[0] * kPageTok, policy);
+            if (np == 2) tma_load_2d(dst + kPageTok * row, map, &full[slot], x, page[1] * kPageTok, policy);
           }
         }
       }
@@ -383,108 +445,103 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       for (int i = max(0, nsc - kScaleStages); i < nsc; ++i)
         mbar_wait(&sc_full[i % kScaleStages], (uint32_t)(i / kScaleStages) & 1u, no_abort);
     }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------- MMA issuer
+  } else if (warp == kQkWarp) {
+    // ------------------------------------------------------ QK: S^T of each tile
     // The whole warp walks and waits; one elected lane issues.  (Issued from a
-    // lane == 0 branch an MMA costs 147 cycles whatever its N, measured;
-    // elected, with operands in uniform registers, 42 at N = 32, 50 at 64, 66
-    // at 128: the operands' shared-memory reads.)
+    // lane == 0 branch, or with operands that the compiler does not know to be
+    // warp-uniform, an MMA costs 147 cycles whatever its N, measured; elected
+    // and uniform 42 at N = 32, 50 at 64, 66 at 128: its shared-memory reads.)
+    // QK and PV have a warp each, so that neither waits behind the other's
+    // operands.
     if (count > 0) {
-      constexpr uint32_t kMN = (1u << 15) | (1u << 16);  // A and B MN-major
       constexpr uint32_t ID_QK = idesc_e4m3_f32(128, 2 * HB), ID_QR = idesc_bf16_f32(128, HB, 0, 0);
-      constexpr uint32_t ID_PV = idesc_e4m3_f32(128, HB) | kMN;
-      // operands' descriptors but for the slab's address
       const uint64_t d_q8 = smem_desc(smem_base + S::OFF_Q8, 16, 1024, kSwizzle128B);
       const uint64_t d_qr = P == 64 ? smem_desc(smem_base + S::OFF_QR, 16, 1024, kSwizzle128B)
                                     : smem_desc(smem_base + S::OFF_QR, 16, 512, kSwizzle64B);
+      const uint64_t d_slab = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
+      const uint64_t d_rope = P == 64 ? d_slab : smem_desc(smem_base + S::OFF_RING, 16, 512, kSwizzle64B);
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
+      Cursor<NS> at;  // the tile's first slab
+      int seg = 0;
+      bool ok = true;
+#pragma unroll 1
+      for (int n = 0; ok && n < count; ++n) {
+        if (n > 0) w.next();
+        if (n == 0 || w.tile == 0) ok = wait(q_ready, (uint32_t)seg++ & 1u);
+        if (ok && n >= 2) ok = wait(&s_free[n & 1], (uint32_t)((n >> 1) - 1) & 1u);
+        if (!ok) break;
+        const uint32_t d = tmem + S::T_S + (uint32_t)uniform(n & 1) * 2 * HB;
+        // latents 0 (its first MMA clears both digits' columns), rope, latents 1 ..
+#pragma unroll
+        for (int step = 0; step < NSLAB; ++step) {
+          const int k = step == 0 ? 1 : step == 1 ? 0 : step;  // slab of the tile, in load order
+          const Cursor<NS> c = at.plus(k);
+          if (!wait(&full[c.slot], c.phase)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t off = (uint32_t)(uniform(c.slot) * S::SLAB) >> 4;
+          if (elect_one()) {
+            if (k == 0) {
+#pragma unroll
+              for (int ks = 0; ks < P / 16; ++ks) mma_bf16_ss(d, d_rope + off + ks * 2, d_qr + ks * 2, ID_QR, 1u);
+              tc_commit(&empty[c.slot]);
+            } else {
+              constexpr uint32_t kSlabQ = 2 * HB * 128 >> 4;
+#pragma unroll
+              for (int ks = 0; ks < 4; ++ks)
+                mma_f8_ss(d, d_slab + off + ks * 2, d_q8 + (k - 1) * kSlabQ + ks * 2, ID_QK, k > 1 || ks > 0 ? 1u : 0u);
+            }
+            if (step == NSLAB - 1) tc_commit(&s_full[n & 1]);
+          }
+        }
+        at.step(NSLAB);
+      }
+      if (!ok) raise_abort(abort, status, kStatusTimeout);
+      // every issued MMA must finish before TMEM and shared memory are released
+      if (elect_one()) tc_commit(&drain[0]);
+      mbar_wait(&drain[0], 0, no_abort);
+    }
+  } else if (warp == kPvWarp) {
+    // --------------------------------------------------- PV: O^T of the segment
+    if (count > 0) {
+      constexpr uint32_t ID_PV = idesc_e4m3_f32(128, HB) | (1u << 15) | (1u << 16);  // A and B MN-major
       // P digits, no swizzle: 16 heads x 8 tokens per 128-byte core matrix,
       // token groups 128 bytes apart, head groups 2048
       const uint64_t d_p = smem_desc(smem_base + S::OFF_P, 128, kTileTok * 16, kSwizzleNone);
       const uint64_t d_slab = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
-      const uint64_t d_rope = P == 64 ? d_slab : smem_desc(smem_base + S::OFF_RING, 16, 512, kSwizzle64B);
-      Cursor<NS> here, ahead;  // first slab of tile n, and of the tile QK is at
       auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
-      auto commit = [&](uint64_t* bar) {
-        if (elect_one()) tc_commit(bar);
-      };
+      Cursor<NS> at;  // the tile's first latent slab
+      at.step(1);
+      int seg = 0;
       bool ok = true;
-      // step 0: latents 0; step 1: rope; steps 2 ..: latents 1 ..
-      auto qk_step = [&](uint32_t buf, int step) {
-        const int k = step == 0 ? 1 : step == 1 ? 0 : step;  // slab of the tile, in load order
-        const Cursor<NS> c = ahead.plus(k);
-        const int slot = c.slot;
-        if (!wait(&full[slot], c.phase)) return false;
+#pragma unroll 1
+      for (int n = 0; ok && n < count; ++n) {
+        if (n > 0) w.next();
+        const bool first = n == 0 || w.tile == 0;  // of its segment
+        if (first && n > 0) ok = wait(o_free, (uint32_t)seg++ & 1u);
+        if (!ok || !wait(p_full, (uint32_t)n & 1u)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t d = tmem + S::T_S + buf * 2 * HB;
-        const uint32_t off = (uint32_t)(slot * S::SLAB) >> 4;
+        int slot[NL];
+#pragma unroll
+        for (int g = 0; g < NL; ++g) slot[g] = uniform(at.plus(g).slot);
         if (elect_one()) {
-          if (k == 0) {
 #pragma unroll
-            for (int ks = 0; ks < P / 16; ++ks) mma_bf16_ss(d, d_rope + off + ks * 2, d_qr + ks * 2, ID_QR, 1u);
-            tc_commit(&empty[slot]);
-          } else {
-            const uint32_t qoff = (uint32_t)((k - 1) * 2 * HB * 128) >> 4;
+          for (int g = 0; g < NL; ++g) {
+            const uint64_t a = d_slab + ((uint32_t)(slot[g] * S::SLAB) >> 4);
+            const uint32_t d = tmem + S::T_O + (uint32_t)(g * HB);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              mma_f8_ss(d, d_slab + off + ks * 2, d_q8 + qoff + ks * 2, ID_QK, k > 1 || ks > 0 ? 1u : 0u);
-          }
-        }
-        return true;
-      };
-      int seg = 0;  // segments whose query was waited for
-      bool first = true;  // tile n begins a segment
-      // n = -1: tile 0's QK alone
-#pragma unroll 1
-      for (int n = -1; ok && n < count; ++n) {
-        const bool more = n + 1 < count;
-        if (n >= 0) {
-          here = ahead;
-          ahead.step(NSLAB);
-          if (more) w.next();
-        }
-        const bool fresh = more && (n < 0 || w.tile == 0);  // tile n + 1 begins a segment
-        const int early = !more || fresh ? 0 : S::LA;       // its QK steps before tile n's PV
-#pragma unroll 1
-        for (int half = 0; ok && half < 2; ++half) {
-          if (half == 1) {
-            if (n >= 0) {
-              ok = wait(p_full, (uint32_t)n & 1u);
-              if (ok && first && seg > 1) ok = wait(o_free, (uint32_t)(seg - 2) & 1u);
-              if (!ok) break;
-              tc_fence_after();
-#pragma unroll 1
-              for (int g = 0; g < NL; ++g) {
-                const int slot = here.plus(1 + g).slot;
-                const uint64_t a = d_slab + ((uint32_t)(slot * S::SLAB) >> 4);
-                const uint32_t d = tmem + S::T_O + g * HB;
-                if (elect_one()) {
-#pragma unroll
-                  for (int ks = 0; ks < kTileTok / 32; ++ks) {
-                    mma_f8_ss(d, a + ks * (4096 >> 4), d_p + ks * (512 >> 4), ID_PV, first && ks == 0 ? 0u : 1u);
-                    mma_f8_ss(d, a + ks * (4096 >> 4), d_p + (S::P_BYTES >> 4) + ks * (512 >> 4), ID_PV, 1u);
-                  }
-                  tc_commit(&empty[slot]);
-                }
-              }
-              commit(pv_done);
+            for (int ks = 0; ks < kTileTok / 32; ++ks) {
+              mma_f8_ss(d, a + ks * (4096 >> 4), d_p + ks * (512 >> 4), ID_PV, first && ks == 0 ? 0u : 1u);
+              mma_f8_ss(d, a + ks * (4096 >> 4), d_p + (S::P_BYTES >> 4) + ks * (512 >> 4), ID_PV, 1u);
             }
-            first = fresh;
-            if (fresh) {
-              ok = wait(q_ready, (uint32_t)seg & 1u);
-              ++seg;
-            }
+            tc_commit(&empty[slot[g]]);
           }
-#pragma unroll 1
-          for (int st = half == 0 ? 0 : early; ok && st < (half == 0 ? early : more ? NSLAB : 0); ++st) {
-            ok = qk_step((uint32_t)(n + 1) & 1u, st);
-            if (ok && st == NSLAB - 1) commit(&s_full[(n + 1) & 1]);
-          }
+          tc_commit(pv_done);
         }
+        at.step(NSLAB);
       }
       if (!ok) raise_abort(abort, status, kStatusTimeout);
-      // every issued MMA must finish before TMEM and shared memory are released
-      commit(drain);
-      mbar_wait(drain, 0, no_abort);
+      if (elect_one()) tc_commit(&drain[1]);
+      mbar_wait(&drain[1], 0, no_abort);
     }
   } else {
     // ------------------------------------------- softmax / accumulate warps
@@ -580,15 +637,18 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     };
 
     // Probabilities and sums are in units of 2^r, r a per-head reference (held
-    // by lane head % HW) that stays within kRefLow .. kRefHigh above each
-    // tile's maximum: a probability then keeps its digits whatever came
-    // before it.  When a tile's maximum leaves that window, the reference
-    // moves (kRefNew above it) and the head's columns of O^T are rescaled in
-    // TMEM; fp32 has the range for both directions (r never falls more than
-    // 2^40 below the largest: what far is out of an fp32 sum's reach).
-    constexpr float kRefNew = 4.0f, kRefHigh = 8.0f, kRefLow = -0.8f;
+    // by lane head % HW) that keeps each tile's largest probability between
+    // 1 and 430: its digits then hold it to 2^-10, and what is smaller than
+    // 2^-4 of the largest to a 2^-14th of it, whatever came before.  When a
+    // tile's maximum leaves that window, the reference moves (to make it 16)
+    // and the head's columns of O^T are rescaled in TMEM; fp32 has the range
+    // for both directions (r never falls more than 2^40 below the largest:
+    // what lies further down is out of an fp32 sum's reach).
+    constexpr float kNew = 4.0f, kHigh = 8.75f, kLow = 0.0f;  // of the tile's maximum, in log2
     float ls[HW];  // softmax sums over this thread's tokens
     float r_ref = 0.0f, r_top = 0.0f;
+    if (lane < HW) mt[lane] = 0.0f;
+    __syncwarp();
     int meet = 0;  // phase of wg_bar
     bool ok = true, first = true;       // first: the tile begins a segment
     bool shared_front = w.tile != 0;    // the segment's sequence began in an earlier run
@@ -612,6 +672,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           sc_phase ^= 1u;
         }
         const float lsig = __log2f(sigma), isig = __frcp_rn(sigma);
+        const uint64_t sigma2 = pair(sigma, sigma), lsig2 = pair(lsig, lsig), isig2 = pair(isig, isig);
         if (!wait(&s_full[n & 1], (uint32_t)(n >> 1) & 1u)) { ok = false; break; }
         tc_fence_after();
         float u[HW];
@@ -624,47 +685,92 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
             tmem_ld(ts + c, s_hi);
             tmem_ld(ts + HB + c, s_lo);
             tmem_ld_wait();
-            auto score = [&](int h, float f) {
-              u[c + h] = fmaf((__uint_as_float(s_hi[h]) + __uint_as_float(s_lo[h])) * sigma, f, lsig);
-            };
 #pragma unroll
             for (int h = 0; h < HC; h += 4) {
-              const float4 f = *reinterpret_cast<const float4*>(fh + wg * HW + c + h);
-              score(h, f.x);
-              score(h + 1, f.y);
-              score(h + 2, f.z);
-              score(h + 3, f.w);
+              const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(fh + wg * HW + c + h);
+              const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(mt + c + h);  // - reference
+              auto score = [&](int i, uint64_t f2, uint64_t r2) {
+                const uint64_t s2 = add2(pair(__uint_as_float(s_hi[i]), __uint_as_float(s_hi[i + 1])),
+                                         pair(__uint_as_float(s_lo[i]), __uint_as_float(s_lo[i + 1])));
+                unpair(fma2(mul2(s2, sigma2), f2, add2(lsig2, r2)), u[c + i], u[c + i + 1]);
+              };
+              score(h, f.x, r.x);
+              score(h + 2, f.y, r.y);
             }
           }
-          if (valid < kTileTok && j >= valid) {
+          tc_fence_before();
+          warp_arrive(&s_free[n & 1]);
+          if (j >= valid) {
 #pragma unroll
             for (int h = 0; h < HW; ++h) u[h] = -INFINITY;
           }
         }
-        // the tile's maximum per head: over the warp's tokens, then the warpgroup's
-        float mine = 0.0f;
+        // the tile's maximum per head (against r), over the warp's tokens and
+        // then the warpgroup's: two heads per register in fp16, whose error
+        // (2^-11 of the value) only matters far from r; lane head % HW gets it
+        uint32_t mx[HW / 2];
 #pragma unroll
-        for (int h = 0; h < HW; ++h) {
-          const float r = redux_max(u[h]);
-          if (lane % HW == h) mine = r;
+        for (int h = 0; h < HW / 2; ++h) mx[h] = pack_half2(u[2 * h], u[2 * h + 1]);
+#pragma unroll
+        for (int o = HW / 2; o >= 2; o >>= 1) {
+          const bool up = (lane & o) != 0;
+#pragma unroll
+          for (int h = 0; h < o / 2; ++h) {
+            const uint32_t give = up ? mx[h] : mx[h + o / 2], keep = up ? mx[h + o / 2] : mx[h];
+            mx[h] = max_half2(keep, __shfl_xor_sync(0xffffffffu, give, o));
+          }
         }
+        mx[0] = max_half2(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], 1));
+#pragma unroll
+        for (int o = HW; o < 32; o <<= 1) mx[0] = max_half2(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+        const float2 two = unpack_half2(mx[0]);
+        float mine = (lane & 1) ? two.y : two.x;
+        const int hl = lane % HW;
         float* red_n = red + ((n & 1) * NWG + wg) * 4 * HW;
         if (lane < HW) red_n[quarter * HW + lane] = mine;
         warp_arrive(&wg_bar[wg]);
         if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
         ++meet;
-        const int hl = lane % HW;
         float t = fmaxf(fmaxf(red_n[hl], red_n[HW + hl]), fmaxf(red_n[2 * HW + hl], red_n[3 * HW + hl]));
-        if (t == -INFINITY) t = 0.0f;
-        r_top = first ? t : fmaxf(r_top, t);
-        const float want = fmaxf(t, r_top - 40.0f);
-        const bool move = first || !(r_ref >= want + kRefLow && r_ref <= want + kRefHigh);
+        if (__any_sync(0xffffffffu, fabsf(t) > 1000.0f)) {
+          // far from the reference (a first tile with large scores, a jump, or
+          // past fp16's range): the maxima once more, in fp32
+#pragma unroll
+          for (int h = 0; h < HW; ++h) {
+            const float r = redux_max(u[h]);
+            if (hl == h) mine = r;
+          }
+          // the warpgroup's four warps are all here: they read the same maxima
+          warp_arrive(&wg_bar[wg]);
+          if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
+          ++meet;
+          if (lane < HW) red_n[quarter * HW + lane] = mine;
+          warp_arrive(&wg_bar[wg]);
+          if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
+          ++meet;
+          t = fmaxf(fmaxf(red_n[hl], red_n[HW + hl]), fmaxf(red_n[2 * HW + hl], red_n[3 * HW + hl]));
+          if (t == -INFINITY) t = 0.0f;
+        }
+        r_top = first ? t + r_ref : fmaxf(r_top, t + r_ref);
+        const float want = fmaxf(t, r_top - 40.0f - r_ref);
+        const bool move = first || !(want >= kLow && want <= kHigh);
         // the previous PV has read P and written O^T
         if (n > 0 && !wait(pv_done, (uint32_t)(n - 1) & 1u)) { ok = false; break; }
         if (uint32_t moved = __ballot_sync(0xffffffffu, move)) {
-          const float to = want + kRefNew;
-          const float f = !move ? 1.0f : fast_exp2(r_ref - to);
-          if (move) r_ref = to;
+          const float by = move ? want - kNew : 0.0f;
+          const float f = fast_exp2(-by);
+          r_ref += by;
+          __syncwarp();
+          if (lane < HW) mt[lane] = by;
+          __syncwarp();
+#pragma unroll
+          for (int h = 0; h < HW; h += 4) {
+            const float4 r = *reinterpret_cast<const float4*>(mt + h);
+            u[h + 0] -= r.x;
+            u[h + 1] -= r.y;
+            u[h + 2] -= r.z;
+            u[h + 3] -= r.w;
+          }
           if (first) {
 #pragma unroll
             for (int h = 0; h < HW; ++h) ls[h] = 0.0f;
@@ -688,22 +794,20 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
             }
             tmem_st_wait();
           }
-          if (lane < HW) mt[lane] = r_ref - 8.0f;
+          __syncwarp();
+          if (lane < HW) mt[lane] = -r_ref;
           __syncwarp();
         }
-        // probabilities in units of 2^(r - 8), their sums and digits
+        // probabilities, their sums and digits
         uint32_t hi[HW / 4], lo[HW / 4];
 #pragma unroll
         for (int h = 0; h < HW; h += 4) {
-          const float4 r = *reinterpret_cast<const float4*>(mt + h);
-          u[h + 0] = fast_exp2(u[h + 0] - r.x);
-          u[h + 1] = fast_exp2(u[h + 1] - r.y);
-          u[h + 2] = fast_exp2(u[h + 2] - r.z);
-          u[h + 3] = fast_exp2(u[h + 3] - r.w);
-          ls[h + 0] = fmaf(u[h + 0], isig, ls[h + 0]);
-          ls[h + 1] = fmaf(u[h + 1], isig, ls[h + 1]);
-          ls[h + 2] = fmaf(u[h + 2], isig, ls[h + 2]);
-          ls[h + 3] = fmaf(u[h + 3], isig, ls[h + 3]);
+          u[h + 0] = fast_exp2(u[h + 0]);
+          u[h + 1] = fast_exp2(u[h + 1]);
+          u[h + 2] = fast_exp2(u[h + 2]);
+          u[h + 3] = fast_exp2(u[h + 3]);
+          unpair(fma2(pair(u[h], u[h + 1]), isig2, pair(ls[h], ls[h + 1])), ls[h], ls[h + 1]);
+          unpair(fma2(pair(u[h + 2], u[h + 3]), isig2, pair(ls[h + 2], ls[h + 3])), ls[h + 2], ls[h + 3]);
           uint32_t a, b2, c, d;
           split_digits(u[h + 0], u[h + 1], a, b2);
           split_digits(u[h + 2], u[h + 3], c, d);
@@ -804,6 +908,10 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       }
       tc_fence_before();
       warp_arrive(o_free);
+      __syncwarp();
+      if (lane < HW) mt[lane] = 0.0f;
+      r_ref = 0.0f;
+      __syncwarp();
       first = true;
       shared_front = false;
       ++n_seg;
