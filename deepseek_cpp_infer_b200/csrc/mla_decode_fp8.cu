@@ -52,7 +52,7 @@ namespace {
 
 constexpr int kTileTok = 128;       // tokens per tile: MMA M
 constexpr int kMaxHeadsPerCta = 64;
-constexpr int kMaxSeqs = 65536;     // prefix array in the scratch
+constexpr int kMaxSeqs = 65536;     // runs of sequences in the scratch
 constexpr int kScaleStages = 4;
 
 template <int R, int P, int HB>
@@ -223,17 +223,17 @@ struct Cursor {
   }
 };
 
-__device__ __forceinline__ void tmem_ld1(uint32_t taddr, uint32_t& r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 // First tile of run i of n over T tiles.
 __device__ __forceinline__ int64_t run_start(int64_t i, int64_t T, int n) { return i * T / n; }
-// The run that holds tile t.
-__device__ __forceinline__ int run_of(int64_t t, int64_t T, int n) { return (int)(((t + 1) * n - 1) / T); }
+// What combine_kernel has to do for a sequence: its first partial's slot and
+// its last run (written by the runs that begin and end it), or one of these.
+constexpr int kSeqEmpty = -1, kSeqWhole = -2;
 
 template <int R, int P, int HB>
 __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
                       const float* __restrict__ scales, int64_t n_blocks, const int32_t* __restrict__ block_table,
                       int max_blocks, const int32_t* __restrict__ seq_lens, int B, int H, int runs, float scale_log2,
                       __nv_bfloat16* __restrict__ out, float* __restrict__ ws_o, float2* __restrict__ ws_ml,
-                      int32_t* __restrict__ prefix, int* __restrict__ status) {
+                      int2* __restrict__ seq_runs, int* __restrict__ status) {
   using S = Shape<R, P, HB>;
   constexpr int NL = S::NL, NS = S::NS, HW = S::HW, NSLAB = S::NSLAB, NWG = S::NWG;
   constexpr int kSmWarps = S::SM_WARPS, kThreads = S::THREADS;
@@ -336,8 +336,9 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       if (w < warp) before += scan[w];
       T += scan[w];
     }
-    run0 = run_start(run, T, runs);
-    count = (int)(run_start(run + 1, T, runs) - run0);
+    const int n_run = min(runs, T);  // no empty runs
+    run0 = run < n_run ? run_start(run, T, n_run) : 0;
+    count = run < n_run ? (int)(run_start(run + 1, T, n_run) - run0) : 0;
     if (count > 0 && run0 >= before && run0 < before + mine) {
       int t = before, b = b0;
 #pragma unroll 1
@@ -349,14 +350,10 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       start[0] = b;
       start[1] = (int)run0 - t;
     }
-    if (blockIdx.x == 0) {  // for combine_kernel
-      int t = before;
+    if (blockIdx.x == 0) {
 #pragma unroll 1
-      for (int b = b0; b < b1; ++b) {
-        prefix[b] = t;
-        t += tiles_of(seq_lens[b], max_blocks);
-      }
-      if (threadIdx.x == 0) prefix[B] = T;
+      for (int b = b0; b < b1; ++b)
+        if (tiles_of(seq_lens[b], max_blocks) == 0) seq_runs[b] = make_int2(kSeqEmpty, 0);
     }
     __syncthreads();
   }
@@ -700,9 +697,9 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           }
           tc_fence_before();
           warp_arrive(&s_free[n & 1]);
-          if (j >= valid) {
+          if (valid < kTileTok) {
 #pragma unroll
-            for (int h = 0; h < HW; ++h) u[h] = -INFINITY;
+            for (int h = 0; h < HW; ++h) u[h] = j < valid ? u[h] : -INFINITY;
           }
         }
         // the tile's maximum per head (against r), over the warp's tokens and
@@ -778,19 +775,21 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
 #pragma unroll
             for (int h = 0; h < HW; ++h) ls[h] *= __shfl_sync(0xffffffffu, f, h);
             tc_fence_after();
-            moved &= 0xffffffffu >> (32 - HW);
 #pragma unroll 1
-            while (moved != 0) {
-              const int h = __ffs(moved) - 1;
-              moved &= moved - 1;
-              const float fh1 = __shfl_sync(0xffffffffu, f, h);
-              uint32_t o[NL];
+            for (int c = 0; c < HW; c += 8) {
+              if (((moved >> c) & 0xffu) == 0) continue;
+              float fs[8];
 #pragma unroll
-              for (int g = 0; g < NL; ++g) tmem_ld1(t_lane + S::T_O + g * HB + wg * HW + h, o[g]);
-              tmem_ld_wait();
+              for (int i = 0; i < 8; ++i) fs[i] = __shfl_sync(0xffffffffu, f, c + i);
+#pragma unroll 1
+              for (int g = 0; g < NL; ++g) {
+                uint32_t o[8];
+                tmem_ld8(t_lane + S::T_O + g * HB + wg * HW + c, o);
+                tmem_ld_wait();
 #pragma unroll
-              for (int g = 0; g < NL; ++g)
-                tmem_st1(t_lane + S::T_O + g * HB + wg * HW + h, __float_as_uint(__uint_as_float(o[g]) * fh1));
+                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fs[i]);
+                tmem_st8(t_lane + S::T_O + g * HB + wg * HW + c, o);
+              }
             }
             tmem_st_wait();
           }
@@ -806,8 +805,6 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           u[h + 1] = fast_exp2(u[h + 1]);
           u[h + 2] = fast_exp2(u[h + 2]);
           u[h + 3] = fast_exp2(u[h + 3]);
-          unpair(fma2(pair(u[h], u[h + 1]), isig2, pair(ls[h], ls[h + 1])), ls[h], ls[h + 1]);
-          unpair(fma2(pair(u[h + 2], u[h + 3]), isig2, pair(ls[h + 2], ls[h + 3])), ls[h + 2], ls[h + 3]);
           uint32_t a, b2, c, d;
           split_digits(u[h + 0], u[h + 1], a, b2);
           split_digits(u[h + 2], u[h + 3], c, d);
@@ -843,6 +840,8 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         tc_fence_before();
         warp_arrive(p_full);
         first = false;
+#pragma unroll
+        for (int h = 0; h < HW; h += 2) unpair(fma2(pair(u[h], u[h + 1]), isig2, pair(ls[h], ls[h + 1])), ls[h], ls[h + 1]);
         if (n + 1 < count) w.next();
       }
       if (!seg_end) continue;
@@ -875,6 +874,11 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       const int hb = h0 + wg * HW;  // first head of this warpgroup
       const bool whole = !shared_front && seq_end;
       const int64_t slot = (int64_t)blockIdx.x * 2 + (n_seg > 0 ? 1 : 0);
+      if (hg == 0 && threadIdx.x == 0) {
+        if (whole) seq_runs[b_now].x = kSeqWhole;
+        else if (!shared_front) seq_runs[b_now].x = run * 2 + (n_seg > 0 ? 1 : 0);
+        if (!whole && seq_end) seq_runs[b_now].y = run;
+      }
       if (lane < HW) {
         mt[lane] = 1.0f / l;
         if (!whole && quarter == 0) ws_ml[slot * HB + wg * HW + lane] = make_float2(r_ref, l);
@@ -936,30 +940,26 @@ constexpr int kCombineWarps = 8;
 
 template <int R, bool kWarpPerHead>
 __global__ void __launch_bounds__(kCombineWarps * 32)
-    combine_kernel(const int32_t* __restrict__ prefix, int B, int H, int HB, int runs,
+    combine_kernel(const int2* __restrict__ seq_runs, int H, int HB, int runs,
                    const float* __restrict__ ws_o, const float2* __restrict__ ws_ml, __nv_bfloat16* __restrict__ out) {
   pdl_wait();
   pdl_launch_dependents();
   constexpr int V = R / 128;  // float4 per lane
   const int warp = (int)warp_id(), lane = (int)lane_id();
   const int b = blockIdx.x, h = kWarpPerHead ? blockIdx.y * kCombineWarps + warp : blockIdx.y;
-  const int64_t t0 = prefix[b], t1 = prefix[b + 1], T = prefix[B];
+  const int2 mine = seq_runs[b];
   __nv_bfloat16* dst = out + ((int64_t)b * H + h) * R + lane * 4;
-  if (t0 == t1) {
+  if (mine.x == kSeqEmpty) {
     if (h < H && (kWarpPerHead || warp == 0)) {
 #pragma unroll
       for (int v = 0; v < V; ++v) *reinterpret_cast<uint2*>(dst + v * 128) = make_uint2(0, 0);
     }
     return;
   }
-  const int i0 = run_of(t0, T, runs), i1 = run_of(t1 - 1, T, runs);
-  if (i0 == i1) return;  // written whole
-  if (kWarpPerHead && h >= H) return;
-  const int64_t cta0 = (int64_t)(h / HB) * runs, hl = h % HB;
-  // the first run's segment of this sequence is its last one: its second
-  // slot, unless the run also begins there
-  const int second = run_start(i0, T, runs) != t0 ? 1 : 0;
-  const bool gaps = T < runs;
+  if (mine.x == kSeqWhole || (kWarpPerHead && h >= H)) return;
+  const int i0 = mine.x >> 1, i1 = mine.y;
+  // partial slots: a run's first segment, then its last
+  const int cta0 = h / HB * runs, hl = h % HB;
   float m = -INFINITY, l = 0.0f;
   float4 o[V];
 #pragma unroll
@@ -967,10 +967,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
   constexpr int kStep = kWarpPerHead ? 1 : kCombineWarps;
 #pragma unroll 4
   for (int i = i0 + (kWarpPerHead ? 0 : warp); i <= i1; i += kStep) {
-    // a run between i0 and i1 may be empty only when there are fewer tiles
-    // than runs; it then wrote nothing
-    if (gaps && run_start(i, T, runs) == run_start(i + 1, T, runs)) continue;
-    const int64_t s = ((cta0 + i) * 2 + (i == i0 ? second : 0)) * HB + hl;
+    const int64_t s = (int64_t)((cta0 + i) * 2 + (i == i0 ? mine.x & 1 : 0)) * HB + hl;
     const float2 ml = ws_ml[s];
     const float mn = fmaxf(m, ml.x), a = fast_exp2(m - mn), c = fast_exp2(ml.x - mn);
     m = mn;
@@ -1020,12 +1017,12 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
   }
 }
 
-// The scratch: the prefix array, then every CTA's two partials.  One size for
+// The scratch: the sequences' runs, then every CTA's two partials.  One size for
 // every call (128 KB a partial at 64 heads x 512 columns), so that captured
 // calls keep their addresses.
 size_t scratch_bytes(int sm) {
   const size_t partials = (size_t)sm * 2 * kMaxHeadsPerCta;
-  return (kMaxSeqs + 64) * sizeof(int32_t) + partials * (512 * sizeof(float) + sizeof(float2));
+  return kMaxSeqs * sizeof(int2) + partials * (512 * sizeof(float) + sizeof(float2));
 }
 
 template <int R, int P, int HB>
@@ -1043,8 +1040,8 @@ int launch(dsb_ctx* ctx, const void* q_lat, const void* q_rope, const void* cach
   if (rc != DSB_OK) return rc;
   const int groups = (H + HB - 1) / HB;
   const int runs = std::max(1, ctx->sm_count / groups);
-  auto* prefix = static_cast<int32_t*>(ctx->mla8);
-  auto* ws_ml = reinterpret_cast<float2*>(prefix + kMaxSeqs + 64);
+  auto* seq_runs = static_cast<int2*>(ctx->mla8);
+  auto* ws_ml = reinterpret_cast<float2*>(seq_runs + kMaxSeqs);
   auto* ws_o = reinterpret_cast<float*>(ws_ml + (size_t)ctx->sm_count * 2 * kMaxHeadsPerCta);
   auto kern = decode_fp8_kernel<R, P, HB>;
   static std::atomic<bool> attr_set[kMaxDevices];
@@ -1053,10 +1050,10 @@ int launch(dsb_ctx* ctx, const void* q_lat, const void* q_rope, const void* cach
                                map_rope, static_cast<const __nv_bfloat16*>(q_lat),
                                static_cast<const __nv_bfloat16*>(q_rope), scales, n_blocks, block_table, max_blocks,
                                seq_lens, B, H, runs, softmax_scale * 1.4426950408889634f,
-                               static_cast<__nv_bfloat16*>(out), ws_o, ws_ml, prefix, ctx->d_status));
+                               static_cast<__nv_bfloat16*>(out), ws_o, ws_ml, seq_runs, ctx->d_status));
   auto combine = [&](auto kernel, unsigned y) {
-    return launch_pdl(kernel, dim3((unsigned)B, y), kCombineWarps * 32, 0, ctx->stream, prefix, B, H, HB, runs, ws_o,
-                      ws_ml, static_cast<__nv_bfloat16*>(out));
+    return launch_pdl(kernel, dim3((unsigned)B, y), kCombineWarps * 32, 0, ctx->stream, seq_runs, H, HB, runs, ws_o, ws_ml,
+                      static_cast<__nv_bfloat16*>(out));
   };
   // a sequence has about runs / B partials
   if (B >= 32) DSB_CUDA_TRY(ctx, combine(combine_kernel<R, true>, (unsigned)((H + kCombineWarps - 1) / kCombineWarps)));
