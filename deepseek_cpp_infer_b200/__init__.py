@@ -276,18 +276,20 @@ def _ptr(t) -> int:
     return 0 if t is None else int(t.data_ptr())
 
 
-def _need(name: str, t, dtype: str, shape, device: int, inner: int = 0):
-    """Check a tensor argument of the 8-bit cache and prompt-attention calls: type, sizes (None: any), device, and
-    rows laid out without gaps (dimensions before `inner` may have any pitch)."""
-    if str(t.dtype) != "torch." + dtype or len(t.shape) != len(shape) or not t.is_cuda or t.device.index != device:
+def _need(name: str, t, dtype: str, shape: tuple, device: int, inner: int = 0):
+    """Check a tensor argument of the 8-bit cache and prompt-attention calls: type, sizes, device, and rows laid out
+    without gaps (dimensions before `inner` may have any pitch)."""
+    import torch
+
+    if t.dtype is not getattr(torch, dtype) or t.shape != shape or t.get_device() != device:
         raise ValueError(f"{name}: {dtype} {shape} on cuda:{device} wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.is_contiguous():
+        return
     step = 1
-    for i in range(len(shape) - 1, -1, -1):
-        if shape[i] is not None and t.shape[i] != shape[i]:
-            raise ValueError(f"{name}: sizes {shape} wanted, got {tuple(t.shape)}")
-        if i >= inner and t.shape[i] != 1 and t.stride(i) != step and t.numel():
+    for i in range(len(shape) - 1, inner - 1, -1):
+        if shape[i] != 1 and t.stride(i) != step and t.numel():
             raise ValueError(f"{name}: rows must be dense (sizes {tuple(t.shape)}, strides {t.stride()})")
-        step *= t.shape[i]
+        step *= shape[i]
 
 
 class Context:
@@ -432,9 +434,9 @@ class Context:
 
     # ---- 8-bit latent cache: cache uint8 [n_blocks, 64, R + 2P], scales fp32 [n_blocks, 64]
     def _need_cache(self, cache, scales, block_table, R, P):
-        _need("cache", cache, "uint8", (None, 64, R + 2 * P), self.device)
+        _need("cache", cache, "uint8", (cache.shape[0], 64, R + 2 * P), self.device)
         _need("scales", scales, "float32", (cache.shape[0], 64), self.device)
-        _need("block_table", block_table, "int32", (None, None), self.device)
+        _need("block_table", block_table, "int32", (block_table.shape[0], block_table.shape[-1]), self.device)
 
     def kv_norm_rope_append_fp8(self, kv_a, w_norm, q, positions, block_table, H, nope, R, P, eps, theta, cache,
                                 scales, q_rope, seq_ids=None):
@@ -442,9 +444,9 @@ class Context:
         Row b belongs to sequence seq_ids[b] (None: b); a negative position marks padding."""
         B = kv_a.shape[0]
         self._need_cache(cache, scales, block_table, R, P)
-        _need("kv_a", kv_a, "float32", (B, None), self.device, inner=1)
+        _need("kv_a", kv_a, "float32", (B, kv_a.shape[-1]), self.device, inner=1)
         _need("w_norm", w_norm, "float32", (R,), self.device)
-        _need("q", q, "bfloat16", (B, None), self.device, inner=1)
+        _need("q", q, "bfloat16", (B, q.shape[-1]), self.device, inner=1)
         _need("positions", positions, "int32", (B,), self.device)
         _need("q_rope", q_rope, "bfloat16", (B, H, P), self.device)
         if seq_ids is not None:
@@ -474,7 +476,7 @@ class Context:
         T, R = latent.shape
         P = k_rope.shape[1]
         self._need_cache(cache, scales, block_table, R, P)
-        _need("cu_seqlens", cu_seqlens, "int32", (None,), self.device)
+        _need("cu_seqlens", cu_seqlens, "int32", (cu_seqlens.numel(),), self.device)
         _need("latent", latent, "bfloat16", (T, R), self.device, inner=1)
         _need("k_rope", k_rope, "bfloat16", (T, P), self.device, inner=1)
         B = cu_seqlens.shape[0] - 1
@@ -495,7 +497,7 @@ class Context:
             _need(name, t, "bfloat16", (rows, H, dim), self.device, inner=2)
         _need("k_rope", k_rope, "bfloat16", (Tk, P), self.device, inner=1)
         _need("out", out, "bfloat16", (Tq, H, vd), self.device, inner=1)
-        _need("cu_q", cu_q, "int32", (None,), self.device)
+        _need("cu_q", cu_q, "int32", (cu_q.numel(),), self.device)
         _need("cu_k", cu_k, "int32", (cu_q.shape[0],), self.device)
         if lse is not None:
             _need("lse", lse, "float32", (Tq, H), self.device)

@@ -244,7 +244,7 @@ def test_refusals(gpu_ctx):
     def refused(code, *a):
         import torch
 
-        out = torch.empty(10, 2, 128, dtype=torch.bfloat16, device="cuda")
+        out = torch.empty(10, 2, a[4].shape[2], dtype=torch.bfloat16, device="cuda")
         with pytest.raises(DsbError) as e:
             gpu_ctx.mla_prefill(*a, cu_of([10]), cu_of([10]), 10, scale if len(a) == 5 else a[5], out)
         assert e.value.code == code
