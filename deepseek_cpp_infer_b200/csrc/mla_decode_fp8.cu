@@ -46,6 +46,7 @@
 #include "dsb_internal.h"
 #include "dsb_ptx.cuh"
 #include "mla_fp8.cuh"
+#include "packed.cuh"
 
 namespace dsb {
 namespace {
@@ -96,31 +97,6 @@ struct Shape {
 // computed from it stay in uniform registers, and branches on it do not
 // count as divergent (in either case an MMA would cost 3 times as much).
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
-
-// Two floats in one register pair: one instruction for both (fma / add / mul .f32x2).
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 __device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
   uint32_t r;

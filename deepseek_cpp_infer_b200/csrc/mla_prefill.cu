@@ -31,6 +31,7 @@
 
 #include "dsb_internal.h"
 #include "dsb_ptx.cuh"
+#include "packed.cuh"
 
 namespace dsb {
 namespace {
@@ -65,8 +66,6 @@ struct Shape {
   // TMEM columns
   static constexpr uint32_t T_S = 0, T_O = 256;
 };
-
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // Ring slots in load order.  A V tile of two slabs is one MMA operand, so its
 // slots must follow one another: a single last slot is passed over.
@@ -105,11 +104,10 @@ struct Order {
 
 // Item `it`: groups of heads; within a group the last (longest) block of every
 // head first.
-__device__ __forceinline__ bool get_item(const dsb_mla_prefill_args& a, const Order& o, int64_t it, Item* x, bool* bad) {
-  const int64_t per = (int64_t)o.group * o.blocks;
-  const int64_t g = it / per;
-  const int first = (int)(g * o.group), heads = min(o.group, o.pairs - first);
-  const int r = (int)(it - g * per);
+__device__ __forceinline__ bool get_item(const dsb_mla_prefill_args& a, const Order& o, int it, Item* x, bool* bad) {
+  const int per = o.group * o.blocks, g = it / per;
+  const int first = g * o.group, heads = min(o.group, o.pairs - first);
+  const int r = it - g * per;
   const int blk = o.blocks - 1 - r / heads, pair = first + r % heads;
   x->b = pair / a.H;
   x->h = pair % a.H;
@@ -137,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefill_kernel(const __grid_constant__ CUtensorMap map_qn, const __grid_constant__ CUtensorMap map_qr,
                    const __grid_constant__ CUtensorMap map_kn, const __grid_constant__ CUtensorMap map_kr,
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ dsb_mla_prefill_args a,
-                   const __grid_constant__ Order order, int64_t items, float scale_log2, int* __restrict__ status) {
+                   const __grid_constant__ Order order, int items, float scale_log2, int* __restrict__ status) {
   using S = Shape<NOPE, P, VD>;
   constexpr int NN = S::NN, NQ = S::NQ, NV = S::NV, NS = S::NS;
   extern __shared__ uint8_t smem_raw[];
@@ -227,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ring.flip(s);
       return true;
     };
-    for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
       Item x;
       bool bad;
       const bool live = get_item(a, order, it, &x, &bad);
@@ -271,6 +269,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The whole warp walks and waits, one elected lane issues, operands in
     // uniform registers (an MMA issued otherwise costs 147 cycles; so 66).
     DSB_FEW_REGS;
+    if (elect_one()) {
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort); };
     constexpr uint32_t ID_QK = idesc_bf16_f32(128, 128, 0, 0), ID_PV = idesc_bf16_f32(128, VD, 0, 1);
     const uint64_t d_q = smem_desc(smem_base + S::OFF_Q, 16, 1024, kSwizzle128B);
     const uint64_t d_k = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
@@ -288,7 +288,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         k_slot[i] = ring.take(1);
         if (!wait(&full[k_slot[i]], ring.phase(k_slot[i]))) return false;
         ring.flip(k_slot[i]);
-        k_slot[i] = uniform(k_slot[i]);
       }
       tc_fence_after();
       return true;
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto issue_qk = [&](int t) {
       const uint32_t d = tmem + S::T_S + t * 128;
       const uint32_t qo = (uint32_t)(t * NQ * S::SLAB) >> 4;
-      if (elect_one()) {
+      {
 #pragma unroll
         for (int i = 0; i < NN; ++i)
 #pragma unroll
@@ -311,12 +310,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     auto release_k = [&]() {
-      if (elect_one()) {
+      {
 #pragma unroll
         for (int i = 0; i < NQ; ++i) tc_commit(&empty[k_slot[i]]);
       }
     };
-    for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
       Item x;
       bool bad;
       if (!get_item(a, order, it, &x, &bad) || x.steps() == 0) continue;
@@ -328,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = 0; t < 2; ++t)
         if (x.n[t] > 0) issue_qk(t);
       release_k();
-      if (n == 1 && elect_one()) tc_commit(q_empty);
+      if (n == 1) tc_commit(q_empty);
       const int full_keys = x.common(causal);
       for (int s = 0; ok && s < n; ++s) {
         // V of this step
@@ -342,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = wait(&v_safe[n_safe & 3u], (n_safe >> 2) & 1u);
           ++n_safe;
         }
-        const int vs = uniform(v_slot);
+        const int vs = v_slot;
         const bool more = s + 1 < n;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -354,14 +353,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const uint32_t d = tmem + S::T_O + t * 128, p = tmem + S::T_S + t * 128;
             const uint64_t v = d_v + ((uint32_t)(vs * S::SLAB) >> 4);
-            if (elect_one()) {
+            {
 #pragma unroll
               for (int ks = 0; ks < kRows / 16; ++ks)
                 mma_bf16_ts(d, p + ks * 8, v + ks * (2048 >> 4), ID_PV, s > 0 || ks > 0 ? 1u : 0u);
               tc_commit(&pv_done[t]);
             }
           }
-          if (t == 1 && elect_one()) {
+          if (t == 1) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) tc_commit(&empty[vs + i]);
           }
@@ -371,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok && s + 1 < x.n[t]) issue_qk(t);
             if (ok && t == 1) {
               release_k();
-              if (s + 2 == n && elect_one()) tc_commit(q_empty);
+              if (s + 2 == n) tc_commit(q_empty);
             }
           }
         }
@@ -379,15 +378,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (!ok) raise_abort(abort, status, kStatusTimeout);
     // every issued MMA must finish before TMEM and shared memory are released
-    if (elect_one()) tc_commit(drain);
+    tc_commit(drain);
     mbar_wait(drain, 0, no_abort);
+    }
   } else if (warp >= kScanWarp) {
     // ------------------------------------- masked values (each warp one half)
     DSB_FEW_REGS;
     Ring<NS> ring;
     uint32_t n_safe = 0, n_item = 0;
     const int half = warp - kScanWarp;
-    for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
       Item x;
       bool bad;
       if (!get_item(a, order, it, &x, &bad) || x.steps() == 0) continue;
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t ts = tl + S::T_S + t * 128, to = tl + S::T_O + t * 128;
     uint32_t c = 0, n_item = 0;  // steps of this tile; items with keys
-    for (int64_t it = blockIdx.x; ok && it < items; it += gridDim.x) {
+    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
       Item x;
       bool bad;
       if (!get_item(a, order, it, &x, &bad)) continue;
@@ -494,11 +494,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           float q[4] = {v[0], v[1], v[2], v[3]};
           if (scale_log2 >= 0.0f) {
 #pragma unroll
-            for (int e = 4; e < 128; ++e) q[e & 3] = fmaxf(q[e & 3], v[e]);
+            for (int e = 4; e < 124; e += 2) q[(e >> 1) & 3] = max3(q[(e >> 1) & 3], v[e], v[e + 1]);
+            q[0] = max3(q[0], v[124], v[125]);
+            q[1] = max3(q[1], v[126], v[127]);
             top = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
           } else {
 #pragma unroll
-            for (int e = 4; e < 128; ++e) q[e & 3] = fminf(q[e & 3], v[e]);
+            for (int e = 4; e < 124; e += 2) q[(e >> 1) & 3] = min3(q[(e >> 1) & 3], v[e], v[e + 1]);
+            q[0] = min3(q[0], v[124], v[125]);
+            q[1] = min3(q[1], v[126], v[127]);
             top = fminf(fminf(q[0], q[1]), fminf(q[2], q[3]));
           }
         }
@@ -524,20 +528,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         l *= f;
         const float mm = m == -INFINITY ? 0.0f : m;  // a row that has seen no key yet
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint64_t scale2 = pair(scale_log2, scale_log2), minus_m = pair(-mm, -mm);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float p0 = fast_exp2(fmaf(v[32 * k + 2 * e], scale_log2, -mm));
-            const float p1 = fast_exp2(fmaf(v[32 * k + 2 * e + 1], scale_log2, -mm));
-            sum[e & 3] += p0 + p1;
+            float p0, p1;
+            unpair(fma2(pair(v[32 * k + 2 * e], v[32 * k + 2 * e + 1]), scale2, minus_m), p0, p1);
+            p0 = fast_exp2(p0);
+            p1 = fast_exp2(p1);
+            sum[e & 1] = add2(sum[e & 1], pair(p0, p1));
             w[e] = pack_bf16x2(p0, p1);
           }
           tmem_st16(ts + 16 * k, w);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        {
+          float s0, s1;
+          unpair(add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
+        }
         tmem_st_wait();
         tc_fence_before();
         warp_arrive(&p_full[t]);
@@ -635,6 +646,9 @@ int launch(dsb_ctx* ctx, const dsb_mla_prefill_args& a) {
   // values are read from HBM once and from L2 by the other blocks
   o.group = std::min(o.pairs, std::max(1, (2 * ctx->sm_count + o.blocks - 1) / o.blocks));
   const int64_t items = (int64_t)o.pairs * o.blocks;
+  if (items >= (int64_t)1 << 30)
+    return fail(ctx, DSB_EUNSUPPORTED, "dsb_mla_prefill: %d sequences x %d heads x %d blocks of queries", a.B, a.H,
+                o.blocks);
   auto kern = prefill_kernel<NOPE, P, VD>;
   static std::atomic<bool> attr_set[kMaxDevices];
   if (int rc = smem_attr_once(ctx, kern, S::SMEM_BYTES, attr_set); rc != DSB_OK) return rc;
@@ -642,7 +656,7 @@ int launch(dsb_ctx* ctx, const dsb_mla_prefill_args& a) {
   const float scale_log2 = a.softmax_scale == 0.0f ? 1e-37f : a.softmax_scale * 1.4426950408889634f;
   const unsigned grid = (unsigned)std::min<int64_t>(items, ctx->sm_count);
   DSB_CUDA_TRY(ctx, launch_pdl(kern, dim3(grid), kThreads, S::SMEM_BYTES, ctx->stream, m[0], m[1], m[2], m[3], m[4], a,
-                               o, items, scale_log2, ctx->d_status));
+                               o, (int)items, scale_log2, ctx->d_status));
   ctx->stats.kernel_launches++;
   return DSB_OK;
 }
