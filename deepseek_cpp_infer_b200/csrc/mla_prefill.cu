@@ -441,27 +441,39 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           const int valid = min(kRows, x.lk - s * kRows);
           // this warp's 64 (VD = 64: 32) value columns: a row's 16-byte chunks
-          constexpr int CH = VD / 2 / 8;  // chunks per row and warp
-          for (int e = lane; e < kRows * CH; e += 32) {
-            const int row = e / CH, chunk = half * CH + e % CH, c = chunk % 8;
-            uint4* at = reinterpret_cast<uint4*>(smem + S::OFF_RING + (v_slot + chunk / 8) * S::SLAB + row * 128 +
-                                                 ((c ^ (row & 7)) * 16));
-            if (row >= valid) {
-              *at = make_uint4(0, 0, 0, 0);
-              continue;
-            }
-            const uint4 v = *at;
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            bool hit = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              hit |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
-            if (hit) {
+          constexpr int CH = VD / 2 / 8;        // chunks per row and warp
+          constexpr int PER = kRows * CH / 32;  // and per lane
+          auto chunk_at = [&](int k) {
+            const int e = lane + 32 * k, row = e / CH, chunk = half * CH + e % CH, c = chunk % 8;
+            return reinterpret_cast<uint4*>(smem + S::OFF_RING + (v_slot + chunk / 8) * S::SLAB + row * 128 +
+                                            ((c ^ (row & 7)) * 16));
+          };
+          // an exponent of all ones carries into the sign bit (two bf16 a word)
+          auto non_finite = [](uint32_t w) { return ((w & 0x7fff7fffu) + 0x00800080u) & 0x80008000u; };
+          uint32_t hits = 0;
+#pragma unroll 8
+          for (int k = 0; k < PER; ++k) {
+            const uint4 v = *chunk_at(k);
+            hits |= non_finite(v.x) | non_finite(v.y) | non_finite(v.z) | non_finite(v.w);
+          }
+          if (__any_sync(0xffffffffu, hits != 0) || valid < kRows) {
+#pragma unroll 1
+            for (int k = 0; k < PER; ++k) {
+              const int e = lane + 32 * k, row = e / CH, chunk = half * CH + e % CH;
+              uint4* at = chunk_at(k);
+              if (row >= valid) {
+                *at = make_uint4(0, 0, 0, 0);
+                continue;
+              }
+              const uint4 v = *at;
+              uint32_t w[4] = {v.x, v.y, v.z, v.w};
+              if ((non_finite(w[0]) | non_finite(w[1]) | non_finite(w[2]) | non_finite(w[3])) == 0) continue;
+#pragma unroll 1
               for (int i = 0; i < 8; ++i) {
-                const uint32_t half_word = (w[i / 2] >> (16 * (i & 1))) & 0xffffu;
-                if ((half_word & 0x7f80u) != 0x7f80u) continue;
+                const uint32_t value = (w[i / 2] >> (16 * (i & 1))) & 0xffffu;
+                if ((value & 0x7f80u) != 0x7f80u) continue;
                 const int col = chunk * 8 + i;
-                const uint32_t kind = (half_word & 0x7fu) != 0 ? kNan : (half_word & 0x8000u) != 0 ? kMinusInf : kPlusInf;
+                const uint32_t kind = (value & 0x7fu) != 0 ? kNan : (value & 0x8000u) != 0 ? kMinusInf : kPlusInf;
                 const uint32_t key = (uint32_t)(s * kRows + row) << 3;
                 uint32_t old = word[col], now;
                 do {
