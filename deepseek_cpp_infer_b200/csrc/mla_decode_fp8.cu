@@ -420,20 +420,19 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     }
   } else if (warp == kQkWarp) {
     // ------------------------------------------------------ QK: S^T of each tile
-    // The whole warp walks and waits; one elected lane issues.  (Issued from a
-    // lane == 0 branch, or with operands that the compiler does not know to be
-    // warp-uniform, an MMA costs 147 cycles whatever its N, measured; elected
-    // and uniform 42 at N = 32, 50 at 64, 66 at 128: its shared-memory reads.)
-    // QK and PV have a warp each, so that neither waits behind the other's
-    // operands.
-    if (count > 0) {
+    // One elected lane runs the role.  (Issued from a lane == 0 branch, or by a
+    // warp with operands that the compiler does not know to be uniform, an MMA
+    // costs 147 cycles whatever its N, measured; elected 42 at N = 32, 50 at
+    // 64, 66 at 128: its shared-memory reads.)  QK and PV have a warp each, so
+    // that neither waits behind the other's operands.
+    if (count > 0 && elect_one()) {
       constexpr uint32_t ID_QK = idesc_e4m3_f32(128, 2 * HB), ID_QR = idesc_bf16_f32(128, HB, 0, 0);
       const uint64_t d_q8 = smem_desc(smem_base + S::OFF_Q8, 16, 1024, kSwizzle128B);
       const uint64_t d_qr = P == 64 ? smem_desc(smem_base + S::OFF_QR, 16, 1024, kSwizzle128B)
                                     : smem_desc(smem_base + S::OFF_QR, 16, 512, kSwizzle64B);
       const uint64_t d_slab = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
       const uint64_t d_rope = P == 64 ? d_slab : smem_desc(smem_base + S::OFF_RING, 16, 512, kSwizzle64B);
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort); };
       Cursor<NS> at;  // the tile's first slab
       int seg = 0;
       bool ok = true;
@@ -443,7 +442,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         if (n == 0 || w.tile == 0) ok = wait(q_ready, (uint32_t)seg++ & 1u);
         if (ok && n >= 2) ok = wait(&s_free[n & 1], (uint32_t)((n >> 1) - 1) & 1u);
         if (!ok) break;
-        const uint32_t d = tmem + S::T_S + (uint32_t)uniform(n & 1) * 2 * HB;
+        const uint32_t d = tmem + S::T_S + (uint32_t)(n & 1) * 2 * HB;
         // latents 0 (its first MMA clears both digits' columns), rope, latents 1 ..
 #pragma unroll
         for (int step = 0; step < NSLAB; ++step) {
@@ -451,8 +450,8 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           const Cursor<NS> c = at.plus(k);
           if (!wait(&full[c.slot], c.phase)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t off = (uint32_t)(uniform(c.slot) * S::SLAB) >> 4;
-          if (elect_one()) {
+          const uint32_t off = (uint32_t)(c.slot * S::SLAB) >> 4;
+          {
             if (k == 0) {
 #pragma unroll
               for (int ks = 0; ks < P / 16; ++ks) mma_bf16_ss(d, d_rope + off + ks * 2, d_qr + ks * 2, ID_QR, 1u);
@@ -470,18 +469,18 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       }
       if (!ok) raise_abort(abort, status, kStatusTimeout);
       // every issued MMA must finish before TMEM and shared memory are released
-      if (elect_one()) tc_commit(&drain[0]);
+      tc_commit(&drain[0]);
       mbar_wait(&drain[0], 0, no_abort);
     }
   } else if (warp == kPvWarp) {
     // --------------------------------------------------- PV: O^T of the segment
-    if (count > 0) {
+    if (count > 0 && elect_one()) {
       constexpr uint32_t ID_PV = idesc_e4m3_f32(128, HB) | (1u << 15) | (1u << 16);  // A and B MN-major
       // P digits, no swizzle: 16 heads x 8 tokens per 128-byte core matrix,
       // token groups 128 bytes apart, head groups 2048
       const uint64_t d_p = smem_desc(smem_base + S::OFF_P, 128, kTileTok * 16, kSwizzleNone);
       const uint64_t d_slab = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort); };
       Cursor<NS> at;  // the tile's first latent slab
       at.step(1);
       int seg = 0;
@@ -495,8 +494,8 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         tc_fence_after();
         int slot[NL];
 #pragma unroll
-        for (int g = 0; g < NL; ++g) slot[g] = uniform(at.plus(g).slot);
-        if (elect_one()) {
+        for (int g = 0; g < NL; ++g) slot[g] = at.plus(g).slot;
+        {
 #pragma unroll
           for (int g = 0; g < NL; ++g) {
             const uint64_t a = d_slab + ((uint32_t)(slot[g] * S::SLAB) >> 4);
@@ -513,7 +512,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         at.step(NSLAB);
       }
       if (!ok) raise_abort(abort, status, kStatusTimeout);
-      if (elect_one()) tc_commit(&drain[1]);
+      tc_commit(&drain[1]);
       mbar_wait(&drain[1], 0, no_abort);
     }
   } else {
