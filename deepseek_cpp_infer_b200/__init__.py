@@ -279,9 +279,10 @@ def _ptr(t) -> int:
 def _need(name: str, t, dtype: str, shape: tuple, device: int, inner: int = 0):
     """Check a tensor argument of the 8-bit cache and prompt-attention calls: type, sizes, device, and rows laid out
     without gaps (dimensions before `inner` may have any pitch)."""
-    import torch
-
-    if t.dtype is not getattr(torch, dtype) or t.shape != shape or t.get_device() != device:
+    global _torch
+    if _torch is None:
+        import torch as _torch  # the package itself does without it
+    if t.dtype is not getattr(_torch, dtype) or t.shape != shape or t.get_device() != device:
         raise ValueError(f"{name}: {dtype} {shape} on cuda:{device} wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if t.is_contiguous():
         return
@@ -290,6 +291,9 @@ def _need(name: str, t, dtype: str, shape: tuple, device: int, inner: int = 0):
         if shape[i] != 1 and t.stride(i) != step and t.numel():
             raise ValueError(f"{name}: rows must be dense (sizes {tuple(t.shape)}, strides {t.stride()})")
         step *= shape[i]
+
+
+_torch = None
 
 
 class Context:

@@ -485,3 +485,111 @@ def test_refusals(gpu_ctx):
         with pytest.raises(ValueError):
             gpu_ctx.mla_decode_fp8(*args)
     gpu_ctx.sync()
+
+
+# --------------------------------------------------- moving references, streams
+
+
+@pytest.mark.parametrize("H", [16, 64])
+@pytest.mark.parametrize("pattern", ["rising", "falling", "alternating", "spike", "first", "late_sink"])
+def test_decode_scores_move_between_tiles(gpu_ctx, pattern, H):
+    """Per-tile score levels hundreds apart (logits up to 900): the reference of the probabilities moves up, moves
+    down, and past the range in which maxima are compared in half precision.  q_rope is one-hot, so a level is a
+    single exact product."""
+    import torch
+
+    n, R, P = 9 * 128 - 20, 512, 64
+    q_lat, q_rope, cache, scales, table, scale = decode_inputs([n], H, BIG, seed=30)
+    q_lat *= 0.25
+    q_rope.zero_()
+    q_rope[..., 0] = 1.0
+    tile = torch.arange(n, device="cuda") // 128
+    level = {"rising": 100.0 * tile, "falling": 800.0 - 100.0 * tile, "alternating": 900.0 * (tile % 2),
+             "spike": 900.0 * (torch.arange(n, device="cuda") == 600), "first": 12.0 * (torch.arange(n, device="cuda") == 0),
+             "late_sink": 11.0 * (torch.arange(n, device="cuda") == n - 1)}[pattern]
+    kr = torch.zeros(cache.shape[0], 64, P, device="cuda")
+    idx = table[0][(torch.arange(n, device="cuda") // 64)].long()
+    kr[idx, torch.arange(n, device="cuda") % 64, 0] = level / scale
+    cache[..., R:] = (kr / scales[..., None]).bfloat16().view(torch.uint8)
+    out = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, [n], scale)
+    gpu_ctx.sync()
+    check_decode(out, q_lat, q_rope, cache, scales, table, [n], scale)
+
+
+def test_decode_rows_never_written(gpu_ctx):
+    """A cache as it is created (zero codes, zero scales) behind two written rows: they count as zero rows."""
+    import torch
+
+    n = 200
+    q_lat, q_rope, cache, scales, table, scale = decode_inputs([n], 16, BIG, seed=31)
+    page = table[0].long()
+    cache[page[0], 2:] = 0
+    scales[page[0], 2:] = 0
+    cache[page[1:]] = 0
+    scales[page[1:]] = 0
+    out = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, [n], scale)
+    gpu_ctx.sync()
+    check_decode(out, q_lat, q_rope, cache, scales, table, [n], scale)
+
+
+def test_decode_two_contexts_at_once(gpu_ctx):
+    """Two contexts on two streams, calls in flight together: each has its own scratch."""
+    import torch
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [Context(0) for _ in range(2)]
+    cases = [decode_inputs([5000, 300], 64, BIG, seed=32), decode_inputs([40, 7000, 129], 16, BIG, seed=33)]
+    lens = [[5000, 300], [40, 7000, 129]]
+    dev = [torch.tensor(l, dtype=torch.int32, device="cuda") for l in lens]
+    outs = [torch.empty_like(c[0]) for c in cases]
+    torch.cuda.synchronize()
+    for c, s in zip(ctxs, streams):
+        c.set_stream(s.cuda_stream)
+    for _ in range(20):
+        for i in range(2):
+            ctxs[i].mla_decode_fp8(*cases[i][:5], dev[i], cases[i][5], outs[i])
+    for i in range(2):
+        ctxs[i].sync()
+        check_decode(outs[i], *cases[i][:5], lens[i], cases[i][5])
+        ctxs[i].close()
+
+
+def test_decode_growing_batches_on_one_context(gpu_ctx):
+    """The same context with very different calls in a row: nothing of an earlier call is left in the scratch."""
+    for lens, H in (([3000] * 3, 128), ([1] * 200, 16), ([0, 0, 5], 64), ([9000], 17), ([64] * 33, 128)):
+        x = decode_inputs(lens, H, BIG, seed=34)
+        out = run_decode(gpu_ctx, *x[:5], lens, x[5])
+        gpu_ctx.sync()
+        check_decode(out, *x[:5], lens, x[5])
+
+
+def test_append_captured_and_replayed(gpu_ctx):
+    import torch
+
+    R, P, nope = shape = BIG
+    H, rows = 16, 5
+    stream, ctx = torch.cuda.Stream(), Context(0)
+    ctx.set_stream(stream.cuda_stream)
+    table, n_blocks = ref.make_table([300] * rows, seed=40)
+    kv, w, q = append_case(rows, H, shape, seed=41)
+    pos = torch.tensor([0, 10, 64, 299, 128], dtype=torch.int32, device="cuda")
+    cache = torch.full((n_blocks, 64, R + 2 * P), 0xA5, dtype=torch.uint8, device="cuda")
+    scales = torch.full((n_blocks, 64), -7.0, device="cuda")
+    q_rope = torch.full((rows, H, P), -7.0, dtype=torch.bfloat16, device="cuda")
+    args = (kv, w, q, pos, table, H, nope, R, P, EPS, THETA, cache, scales, q_rope)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ctx.kv_norm_rope_append_fp8(*args)
+    for p in ([0, 10, 64, 299, 128], [1, -1, 65, 200, 7]):
+        pos.copy_(torch.tensor(p, dtype=torch.int32))
+        cache.fill_(0xA5)
+        scales.fill_(-7.0)
+        q_rope.fill_(-7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_append(kv, w, q, pos, torch.arange(rows, device="cuda"), table, H, shape, cache, scales, q_rope)
+    ctx.sync()
+    del graph
+    ctx.close()

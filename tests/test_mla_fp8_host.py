@@ -1,0 +1,79 @@
+"""Host-side checks of the 8-bit latent cache and prompt-attention entry
+points: no GPU is used."""
+
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+
+import deepseek_cpp_infer_b200 as dsb
+import mla_fp8_ref as ref
+
+
+def test_null_context_is_refused():
+    l = dsb.lib()
+    z = ctypes.c_void_p()
+    assert l.dsb_mla_decode_fp8(z, z, z, z, z, 1, z, 1, z, 1, 16, 512, 64, 1.0, z) == dsb.DSB_EINVAL
+    assert l.dsb_kv_norm_rope_append_fp8(z, z, 576, z, z, 16 * 192, z, z, z, 1, 1, 1, 16, 128, 512, 64, 1e-6, 1e4, z, z, 1,
+                                         z) == dsb.DSB_EINVAL
+    assert l.dsb_mla_cache_read_fp8(z, z, z, 1, z, 1, z, 1, 1, 512, 64, z, 512, z, 64) == dsb.DSB_EINVAL
+    assert l.dsb_mla_prefill(z, ctypes.byref(dsb.MlaPrefillArgs())) == dsb.DSB_EINVAL
+
+
+def test_prefill_args_match_the_header(tmp_path):
+    names = [n for n, _ in dsb.MlaPrefillArgs._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "dsb/dsb.h"\nint main(void) {\n'
+                   + "".join(f'  printf("%zu ", offsetof(dsb_mla_prefill_args, {n}));\n' for n in names)
+                   + '  printf("%zu\\n", sizeof(dsb_mla_prefill_args));\n  return 0;\n}\n')
+    inc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    exe = tmp_path / "layout"
+    subprocess.run(["gcc", "-std=c99", f"-I{inc}", str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
+    want = [getattr(dsb.MlaPrefillArgs, n).offset for n in names] + [ctypes.sizeof(dsb.MlaPrefillArgs)]
+    assert got == want
+
+
+def _e4m3_table():
+    """All 256 e4m3 values from the format's definition."""
+    v = np.zeros(256)
+    for c in range(256):
+        s, e, m = c >> 7, (c >> 3) & 15, c & 7
+        x = (m / 8) * 2.0 ** -6 if e == 0 else (1 + m / 8) * 2.0 ** (e - 7)
+        v[c] = np.nan if (e, m) == (15, 7) else (-x if s else x)
+    return v
+
+
+def test_reference_quantiser():
+    """Codes are the nearest e4m3 values of c / scale; the scale is the least power of two that keeps 448."""
+    import torch
+
+    rng = np.random.default_rng(0)
+    c = rng.standard_normal((40, 128)) * np.exp(rng.uniform(-20, 20, (40, 1)))
+    c[0] = 0
+    c[1, 3], c[1, 4:] = 448 * 2.0 ** 5, 1.0  # amax on the border
+    c[2, :] = np.minimum(c[2], 0.1)
+    c[2, 0] = 448 * 2.0 ** 5 * (1 + 2.0 ** -20)  # and just above it
+    codes, scale = ref.quantise(torch.from_numpy(c))
+    scale = scale.double().numpy()
+    assert scale[0] == 1 and scale[1] == 2.0 ** 5 and scale[2] == 2.0 ** 6
+    amax = np.abs(c).max(1)
+    assert (amax <= 448 * scale * (1 + 1e-7))[1:].all() and (amax > 224 * scale * (1 - 1e-7))[1:].all()
+    table = _e4m3_table()
+    finite = np.sort(np.unique(table[np.isfinite(table)]))
+    x = c / scale[:, None]
+    near = finite[np.abs(finite[None, None] - x[..., None]).argmin(-1)]
+    got = table[codes.numpy()]
+    assert (np.abs(got - x) <= np.abs(near - x) + 1e-6 * np.abs(x)).all()
+
+
+def test_every_cached_value_is_exact_in_bf16():
+    """An e4m3 value has 4 significant bits and the scale is a power of two."""
+    import torch
+
+    table = torch.from_numpy(_e4m3_table()).float()
+    table = table[torch.isfinite(table)]
+    for e in (-64, -17, -1, 0, 9, 64):
+        v = table * 2.0 ** e
+        assert torch.equal(v.bfloat16().float(), v)
