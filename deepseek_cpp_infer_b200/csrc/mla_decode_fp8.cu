@@ -104,6 +104,12 @@ __device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
   return r;
 }
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 __device__ __forceinline__ float redux_max(float v) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
@@ -132,7 +138,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// Bring a box into L2 ahead of its load.
+// Bring bytes (address and size multiples of 16) or a box into L2 ahead of their load.
+__device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y)
                : "memory");
@@ -351,6 +361,13 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       bool ok = true;
       for (int n = 0; ok && n < count; ++n) {
         if (n > 0) w.next();
+        if ((n == 0 || w.tile == 0) && w.ntile - w.tile < count - n && w.b + 1 < B && elect_one()) {
+          // the next sequence's queries into L2
+          const int64_t row = (int64_t)(w.b + 1) * H + hg * HB;
+          const int rows = min(HB, H - hg * HB);
+          prefetch_l2(q_lat + row * R, rows * R * 2);
+          prefetch_l2(q_rope + row * P, rows * P * 2);
+        }
         if (at == 32 || w.tile == 0) {
           const int p = w.tile * 2 + lane;
           pages = 0;
@@ -564,22 +581,28 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         const uint32_t (&x)[CPL / 2] = xs[q];
         const uint4 r = rs[q];
         const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
-        float am = 0.0f, rm = 0.0f;
+        uint32_t am = 0, rm = 0;  // magnitudes, two bf16 at once: their order is that of the bits
 #pragma unroll
-        for (int i = 0; i < CPL / 2; ++i) am = fmaxf(am, fmaxf(fabsf(bf16lo_to_f32(x[i])), fabsf(bf16hi_to_f32(x[i]))));
+        for (int i = 0; i < CPL / 2; ++i) am = max_u16x2(am, x[i] & 0x7fff7fffu);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rm = fmaxf(rm, fmaxf(fabsf(bf16lo_to_f32(rr[i])), fabsf(bf16hi_to_f32(rr[i]))));
+        for (int i = 0; i < 4; ++i) rm = max_u16x2(rm, rr[i] & 0x7fff7fffu);
+        const float al = __uint_as_float(max(am & 0xffff0000u, am << 16));
+        const float ar = __uint_as_float(max(rm & 0xffff0000u, rm << 16));
         // the latents' scale; a rope part over 64 times larger sets it
         // instead (it is divided by the same factor, in bf16, exactly)
-        const float top = redux_max(fmaxf(am, rm * 0.015625f));
+        const float top = redux_max(fmaxf(al, ar * 0.015625f));
         const int e = min(100, max(-100, top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 7 : 0));
         const float inv = exp2i(-e);
+        const uint64_t inv2 = pair(inv, inv);
         uint32_t hi[CPL / 4], lo[CPL / 4];
 #pragma unroll
         for (int i = 0; i < CPL / 4; ++i) {
           uint32_t a, b2, c, d;
-          split_digits(bf16lo_to_f32(x[2 * i]) * inv, bf16hi_to_f32(x[2 * i]) * inv, a, b2);
-          split_digits(bf16lo_to_f32(x[2 * i + 1]) * inv, bf16hi_to_f32(x[2 * i + 1]) * inv, c, d);
+          float v[4];
+          unpair(mul2(pair(bf16lo_to_f32(x[2 * i]), bf16hi_to_f32(x[2 * i])), inv2), v[0], v[1]);
+          unpair(mul2(pair(bf16lo_to_f32(x[2 * i + 1]), bf16hi_to_f32(x[2 * i + 1])), inv2), v[2], v[3]);
+          split_digits(v[0], v[1], a, b2);
+          split_digits(v[2], v[3], c, d);
           hi[i] = a | (c << 16);
           lo[i] = b2 | (d << 16);
         }
@@ -732,42 +755,40 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           const float by = move ? want - kNew : 0.0f;
           const float f = fast_exp2(-by);
           r_ref += by;
-          __syncwarp();
-          if (lane < HW) mt[lane] = by;
-          __syncwarp();
+          if (!first) tc_fence_after();
 #pragma unroll
-          for (int h = 0; h < HW; h += 4) {
-            const float4 r = *reinterpret_cast<const float4*>(mt + h);
-            u[h + 0] -= r.x;
-            u[h + 1] -= r.y;
-            u[h + 2] -= r.z;
-            u[h + 3] -= r.w;
-          }
-          if (first) {
+          for (int c = 0; c < HW; c += 8) {
+            if (((moved >> c) & 0xffu) == 0) continue;
 #pragma unroll
-            for (int h = 0; h < HW; ++h) ls[h] = 0.0f;
-          } else {
+            for (int i = 0; i < 8; ++i) u[c + i] -= __shfl_sync(0xffffffffu, by, c + i);
+            if (first) {
 #pragma unroll
-            for (int h = 0; h < HW; ++h) ls[h] *= __shfl_sync(0xffffffffu, f, h);
-            tc_fence_after();
+              for (int i = 0; i < 8; ++i) ls[c + i] = 0.0f;
+              continue;
+            }
+            float fs[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              fs[i] = __shfl_sync(0xffffffffu, f, c + i);
+              ls[c + i] *= fs[i];
+            }
+            constexpr int NB = 1;  // blocks read at once
 #pragma unroll 1
-            for (int c = 0; c < HW; c += 8) {
-              if (((moved >> c) & 0xffu) == 0) continue;
-              float fs[8];
+            for (int g = 0; g < NL; g += NB) {
+              const uint32_t at = t_lane + S::T_O + g * HB + wg * HW + c;
+              uint32_t o[NB][8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) fs[i] = __shfl_sync(0xffffffffu, f, c + i);
-#pragma unroll 1
-              for (int g = 0; g < NL; ++g) {
-                uint32_t o[8];
-                tmem_ld8(t_lane + S::T_O + g * HB + wg * HW + c, o);
-                tmem_ld_wait();
+              for (int k = 0; k < NB; ++k) tmem_ld8(at + k * HB, o[k]);
+              tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fs[i]);
-                tmem_st8(t_lane + S::T_O + g * HB + wg * HW + c, o);
+              for (int k = 0; k < NB; ++k) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[k][i] = __float_as_uint(__uint_as_float(o[k][i]) * fs[i]);
+                tmem_st8(at + k * HB, o[k]);
               }
             }
-            tmem_st_wait();
           }
+          if (!first) tmem_st_wait();
           __syncwarp();
           if (lane < HW) mt[lane] = -r_ref;
           __syncwarp();
@@ -861,22 +882,27 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       __syncwarp();
       if (!wait(pv_done, (uint32_t)n & 1u)) { ok = false; break; }
       tc_fence_after();
-      const bool odd = lane & 1;
 #pragma unroll 1
       for (int g = 0; g < NL; ++g) {
         uint32_t o[HW];
         tmem_ld(t_lane + S::T_O + g * HB + wg * HW, o);
         tmem_ld_wait();
         if (whole) {
-          // lanes swap so that each stores two columns of one head
-          __nv_bfloat16* dst = out + ((int64_t)b_now * H + hb + (odd ? 1 : 0)) * R + g * 128 + quarter * 32 + (lane & ~1);
+          // four lanes swap so that each stores four latents of one head
+          const bool s1 = lane & 1, s2 = lane & 2;
+          const int mine = (s1 ? 2 : 0) + (s2 ? 1 : 0);  // of each four heads
+          __nv_bfloat16* dst = out + ((int64_t)b_now * H + hb + mine) * R + g * 128 + (j & ~3);
 #pragma unroll
-          for (int h = 0; h < HW; h += 2) {
-            const float2 il = *reinterpret_cast<const float2*>(mt + h);
-            const float x = __uint_as_float(o[h]) * il.x, y = __uint_as_float(o[h + 1]) * il.y;
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? x : y, 1);
-            if (hb + h + (odd ? 1 : 0) < H)
-              *reinterpret_cast<uint32_t*>(dst + h * R) = odd ? pack_bf16x2(got, y) : pack_bf16x2(x, got);
+          for (int h = 0; h < HW; h += 4) {
+            const float4 il = *reinterpret_cast<const float4*>(mt + h);
+            const uint32_t w01 = pack_bf16x2(__uint_as_float(o[h]) * il.x, __uint_as_float(o[h + 1]) * il.y);
+            const uint32_t w23 = pack_bf16x2(__uint_as_float(o[h + 2]) * il.z, __uint_as_float(o[h + 3]) * il.w);
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, s1 ? w01 : w23, 1);
+            const uint32_t a = s1 ? got : w01, c = s1 ? w23 : got;  // two heads of latents j & ~1 and j | 1
+            const uint32_t x = __byte_perm(a, c, 0x5410), y = __byte_perm(a, c, 0x7632);
+            const uint32_t far = __shfl_xor_sync(0xffffffffu, s2 ? x : y, 2);
+            if (hb + h + mine < H)
+              *reinterpret_cast<uint2*>(dst + h * R) = s2 ? make_uint2(far, y) : make_uint2(x, far);
           }
         } else {
           float* dst = ws_o + (slot * HB + wg * HW) * R + g * 128 + j;
