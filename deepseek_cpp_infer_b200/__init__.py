@@ -276,24 +276,27 @@ def _ptr(t) -> int:
     return 0 if t is None else int(t.data_ptr())
 
 
-def _need(name: str, t, dtype: str, shape: tuple, device: int, inner: int = 0):
-    """Check a tensor argument of the 8-bit cache and prompt-attention calls: type, sizes, device, and rows laid out
-    without gaps (dimensions before `inner` may have any pitch)."""
-    global _torch
-    if _torch is None:
-        import torch as _torch  # the package itself does without it
-    if t.dtype is not getattr(_torch, dtype) or t.shape != shape or t.get_device() != device:
-        raise ValueError(f"{name}: {dtype} {shape} on cuda:{device} wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if t.is_contiguous():
-        return
-    step = 1
-    for i in range(len(shape) - 1, inner - 1, -1):
-        if shape[i] != 1 and t.stride(i) != step and t.numel():
-            raise ValueError(f"{name}: rows must be dense (sizes {tuple(t.shape)}, strides {t.stride()})")
-        step *= shape[i]
+_DTYPES: dict = {}  # torch's types by name; the package itself does without torch
 
 
-_torch = None
+def _need(device: int, *wanted):
+    """Check the tensors of an 8-bit cache or prompt-attention call, each given as (name, tensor, type, sizes, inner):
+    type, sizes, device, and rows laid out without gaps (dimensions before `inner` may have any pitch)."""
+    if not _DTYPES:
+        import torch
+
+        _DTYPES.update((n, getattr(torch, n)) for n in ("uint8", "float32", "int32", "bfloat16"))
+    for name, t, dtype, shape, inner in wanted:
+        if t.dtype is not _DTYPES[dtype] or t.shape != shape or t.get_device() != device:
+            raise ValueError(
+                f"{name}: {dtype} {shape} on cuda:{device} wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.is_contiguous():
+            continue
+        step = 1
+        for i in range(len(shape) - 1, inner - 1, -1):
+            if shape[i] != 1 and t.stride(i) != step and t.numel():
+                raise ValueError(f"{name}: rows must be dense (sizes {tuple(t.shape)}, strides {t.stride()})")
+            step *= shape[i]
 
 
 class Context:
@@ -437,82 +440,80 @@ class Context:
             H, nope, R, P, float(eps), float(theta), _ptr(cache), _ptr(q_rope)))
 
     # ---- 8-bit latent cache: cache uint8 [n_blocks, 64, R + 2P], scales fp32 [n_blocks, 64]
-    def _need_cache(self, cache, scales, block_table, R, P):
-        _need("cache", cache, "uint8", (cache.shape[0], 64, R + 2 * P), self.device)
-        _need("scales", scales, "float32", (cache.shape[0], 64), self.device)
-        _need("block_table", block_table, "int32", (block_table.shape[0], block_table.shape[-1]), self.device)
-
     def kv_norm_rope_append_fp8(self, kv_a, w_norm, q, positions, block_table, H, nope, R, P, eps, theta, cache,
                                 scales, q_rope, seq_ids=None):
         """dsb_kv_norm_rope_append_fp8: rows of kv_a [B, R+P] fp32 into the 8-bit cache, q_rope [B, H, P] rotated.
         Row b belongs to sequence seq_ids[b] (None: b); a negative position marks padding."""
-        B = kv_a.shape[0]
-        self._need_cache(cache, scales, block_table, R, P)
-        _need("kv_a", kv_a, "float32", (B, kv_a.shape[-1]), self.device, inner=1)
-        _need("w_norm", w_norm, "float32", (R,), self.device)
-        _need("q", q, "bfloat16", (B, q.shape[-1]), self.device, inner=1)
-        _need("positions", positions, "int32", (B,), self.device)
-        _need("q_rope", q_rope, "bfloat16", (B, H, P), self.device)
+        B, width = kv_a.shape
+        blocks, (rows, max_blocks) = cache.shape[0], block_table.shape
+        _need(self.device,
+              ("cache", cache, "uint8", (blocks, 64, R + 2 * P), 0), ("scales", scales, "float32", (blocks, 64), 0),
+              ("block_table", block_table, "int32", (rows, max_blocks), 0), ("kv_a", kv_a, "float32", (B, width), 1),
+              ("w_norm", w_norm, "float32", (R,), 0), ("q", q, "bfloat16", (B, q.shape[-1]), 1),
+              ("positions", positions, "int32", (B,), 0), ("q_rope", q_rope, "bfloat16", (B, H, P), 0))
         if seq_ids is not None:
-            _need("seq_ids", seq_ids, "int32", (B,), self.device)
+            _need(self.device, ("seq_ids", seq_ids, "int32", (B,), 0))
         self._check(self._l.dsb_kv_norm_rope_append_fp8(
-            self.h, _ptr(kv_a), kv_a.stride(0), _ptr(w_norm), _ptr(q), q.stride(0), _ptr(positions), _ptr(seq_ids),
-            _ptr(block_table), block_table.shape[0], block_table.shape[1], B, H, nope, R, P, float(eps), float(theta),
-            _ptr(cache), _ptr(scales), cache.shape[0], _ptr(q_rope)))
+            self.h, kv_a.data_ptr(), kv_a.stride(0), w_norm.data_ptr(), q.data_ptr(), q.stride(0),
+            positions.data_ptr(), _ptr(seq_ids), block_table.data_ptr(), rows, max_blocks, B, H, nope, R, P, eps, theta,
+            cache.data_ptr(), scales.data_ptr(), blocks, q_rope.data_ptr()))
 
     def mla_decode_fp8(self, q_lat, q_rope, cache, scales, block_table, seq_lens, softmax_scale, out):
         """dsb_mla_decode_fp8: q_lat [B, H, R], q_rope [B, H, P] bf16, seq_lens int32 [B] on the device -> out [B, H, R]."""
-        B, H, R = q_lat.shape
+        shape = q_lat.shape
+        B, H, R = shape
         P = q_rope.shape[2]
-        self._need_cache(cache, scales, block_table, R, P)
-        _need("q_lat", q_lat, "bfloat16", (B, H, R), self.device)
-        _need("q_rope", q_rope, "bfloat16", (B, H, P), self.device)
-        _need("out", out, "bfloat16", (B, H, R), self.device)
-        _need("seq_lens", seq_lens, "int32", (B,), self.device)
-        if block_table.shape[0] < B:
-            raise ValueError(f"block_table: {block_table.shape[0]} rows for {B} sequences")
+        blocks, (rows, max_blocks) = cache.shape[0], block_table.shape
+        _need(self.device,
+              ("cache", cache, "uint8", (blocks, 64, R + 2 * P), 0), ("scales", scales, "float32", (blocks, 64), 0),
+              ("block_table", block_table, "int32", (rows, max_blocks), 0), ("q_lat", q_lat, "bfloat16", shape, 0),
+              ("q_rope", q_rope, "bfloat16", (B, H, P), 0), ("out", out, "bfloat16", shape, 0),
+              ("seq_lens", seq_lens, "int32", (B,), 0))
+        if rows < B:
+            raise ValueError(f"block_table: {rows} rows for {B} sequences")
         self._check(self._l.dsb_mla_decode_fp8(
-            self.h, _ptr(q_lat), _ptr(q_rope), _ptr(cache), _ptr(scales), cache.shape[0], _ptr(block_table),
-            block_table.shape[1], _ptr(seq_lens), B, H, R, P, float(softmax_scale), _ptr(out)))
+            self.h, q_lat.data_ptr(), q_rope.data_ptr(), cache.data_ptr(), scales.data_ptr(), blocks,
+            block_table.data_ptr(), max_blocks, seq_lens.data_ptr(), B, H, R, P, softmax_scale, out.data_ptr()))
 
     def mla_cache_read_fp8(self, cache, scales, block_table, cu_seqlens, latent, k_rope):
         """dsb_mla_cache_read_fp8: cached tokens as bf16 rows of latent [T, R] and k_rope [T, P]; cu_seqlens [B + 1]."""
         T, R = latent.shape
         P = k_rope.shape[1]
-        self._need_cache(cache, scales, block_table, R, P)
-        _need("cu_seqlens", cu_seqlens, "int32", (cu_seqlens.numel(),), self.device)
-        _need("latent", latent, "bfloat16", (T, R), self.device, inner=1)
-        _need("k_rope", k_rope, "bfloat16", (T, P), self.device, inner=1)
-        B = cu_seqlens.shape[0] - 1
-        if block_table.shape[0] < B:
-            raise ValueError(f"block_table: {block_table.shape[0]} rows for {B} sequences")
+        blocks, (rows, max_blocks), B = cache.shape[0], block_table.shape, cu_seqlens.numel() - 1
+        _need(self.device,
+              ("cache", cache, "uint8", (blocks, 64, R + 2 * P), 0), ("scales", scales, "float32", (blocks, 64), 0),
+              ("block_table", block_table, "int32", (rows, max_blocks), 0),
+              ("cu_seqlens", cu_seqlens, "int32", (B + 1,), 0), ("latent", latent, "bfloat16", (T, R), 1),
+              ("k_rope", k_rope, "bfloat16", (T, P), 1))
+        if rows < B:
+            raise ValueError(f"block_table: {rows} rows for {B} sequences")
         self._check(self._l.dsb_mla_cache_read_fp8(
-            self.h, _ptr(cache), _ptr(scales), cache.shape[0], _ptr(block_table), block_table.shape[1],
-            _ptr(cu_seqlens), B, T, R, P, _ptr(latent), latent.stride(0), _ptr(k_rope), k_rope.stride(0)))
+            self.h, cache.data_ptr(), scales.data_ptr(), blocks, block_table.data_ptr(), max_blocks,
+            cu_seqlens.data_ptr(), B, T, R, P, latent.data_ptr(), latent.stride(0), k_rope.data_ptr(),
+            k_rope.stride(0)))
 
     def mla_prefill(self, q_nope, q_rope, k_nope, k_rope, v, cu_q, cu_k, max_q, softmax_scale, out, causal=True,
                     lse=None):
         """dsb_mla_prefill on bf16 tensors [T, H, dim] (k_rope [T, P]) of any token and head pitch; out [Tq, H, vd]
         with dense heads; cu_q, cu_k int32 [B + 1]."""
         Tq, H, nope = q_nope.shape
-        Tk, P, vd = k_nope.shape[0], q_rope.shape[2], v.shape[2]
-        for name, t, rows, dim in (("q_nope", q_nope, Tq, nope), ("q_rope", q_rope, Tq, P), ("k_nope", k_nope, Tk, nope),
-                                   ("v", v, Tk, vd)):
-            _need(name, t, "bfloat16", (rows, H, dim), self.device, inner=2)
-        _need("k_rope", k_rope, "bfloat16", (Tk, P), self.device, inner=1)
-        _need("out", out, "bfloat16", (Tq, H, vd), self.device, inner=1)
-        _need("cu_q", cu_q, "int32", (cu_q.numel(),), self.device)
-        _need("cu_k", cu_k, "int32", (cu_q.shape[0],), self.device)
+        Tk, P, vd, n = k_nope.shape[0], q_rope.shape[2], v.shape[2], cu_q.numel()
+        _need(self.device,
+              ("q_nope", q_nope, "bfloat16", (Tq, H, nope), 2), ("q_rope", q_rope, "bfloat16", (Tq, H, P), 2),
+              ("k_nope", k_nope, "bfloat16", (Tk, H, nope), 2), ("v", v, "bfloat16", (Tk, H, vd), 2),
+              ("k_rope", k_rope, "bfloat16", (Tk, P), 1), ("out", out, "bfloat16", (Tq, H, vd), 1),
+              ("cu_q", cu_q, "int32", (n,), 0), ("cu_k", cu_k, "int32", (n,), 0))
         if lse is not None:
-            _need("lse", lse, "float32", (Tq, H), self.device)
+            _need(self.device, ("lse", lse, "float32", (Tq, H), 0))
         a = MlaPrefillArgs(
-            q_nope=_ptr(q_nope), ld_q_nope=q_nope.stride(0), hd_q_nope=q_nope.stride(1),
-            q_rope=_ptr(q_rope), ld_q_rope=q_rope.stride(0), hd_q_rope=q_rope.stride(1),
-            k_nope=_ptr(k_nope), ld_k_nope=k_nope.stride(0), hd_k_nope=k_nope.stride(1),
-            k_rope=_ptr(k_rope), ld_k_rope=k_rope.stride(0), v=_ptr(v), ld_v=v.stride(0), hd_v=v.stride(1),
-            cu_q=_ptr(cu_q), cu_k=_ptr(cu_k), B=cu_q.shape[0] - 1, Tq=Tq, Tk=Tk, max_q=int(max_q), H=H,
-            nope=nope, P=P, vd=vd, causal=int(causal), softmax_scale=float(softmax_scale),
-            out=_ptr(out), ld_out=out.stride(0), lse=_ptr(lse),
+            q_nope=q_nope.data_ptr(), ld_q_nope=q_nope.stride(0), hd_q_nope=q_nope.stride(1),
+            q_rope=q_rope.data_ptr(), ld_q_rope=q_rope.stride(0), hd_q_rope=q_rope.stride(1),
+            k_nope=k_nope.data_ptr(), ld_k_nope=k_nope.stride(0), hd_k_nope=k_nope.stride(1),
+            k_rope=k_rope.data_ptr(), ld_k_rope=k_rope.stride(0),
+            v=v.data_ptr(), ld_v=v.stride(0), hd_v=v.stride(1),
+            cu_q=cu_q.data_ptr(), cu_k=cu_k.data_ptr(), B=n - 1, Tq=Tq, Tk=Tk, max_q=int(max_q), H=H,
+            nope=nope, P=P, vd=vd, causal=int(causal), softmax_scale=softmax_scale,
+            out=out.data_ptr(), ld_out=out.stride(0), lse=_ptr(lse),
         )
         self._check(self._l.dsb_mla_prefill(self.h, ctypes.byref(a)))
 
