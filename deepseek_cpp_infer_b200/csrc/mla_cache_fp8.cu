@@ -181,6 +181,7 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int lane = (int)lane_id();
   const int64_t t0 = ((int64_t)blockIdx.x * kWarps + warp_id()) * kReadRows;
   const int64_t end = min(T, (int64_t)cu[B]);
+  if (t0 == 0 && lane == 0 && cu[B] > T) atomicCAS(status, 0, kStatusBadInput);
   if (t0 >= end) return;
   int lo = 0, hi = B;  // the last sequence that starts at or before t0
   while (hi - lo > 1) {

@@ -15,12 +15,13 @@
 // a power of two per head) is split into hi = e4m3(q / a) and lo = e4m3(q / a
 // - hi), exact down to 2^-18 of the head's largest value.  hi and lo are
 // separate columns of one MMA (N = 2 heads), summed in fp32.  Probabilities
-// are split the same way (8 significant bits, like bf16), in units of their
-// own tile's maximum: each tile's O^T is a fresh accumulator that is added to
-// fp32 registers with the tile's weight, so that thousands of small
-// probabilities behind one large one (an attention sink) keep their digits.
+// are split the same way (8 significant bits, like bf16) in units of a moving
+// reference per head that keeps every tile's largest within the digits' range
+// (see kLow), so that thousands of small probabilities behind one large one
+// (an attention sink) keep their digits.  O^T accumulates in TMEM in fp32 and is
+// rescaled there when the reference moves.
 // The token's scale joins its probability: with u = s log2(e) + log2(sigma),
-// p' = 2^(u - max u) carries sigma, and the softmax sum takes p' / sigma.
+// p' = 2^(u - r) carries sigma, and the softmax sum takes p' / sigma.
 //
 // Work.  Sequences' tiles in order, cut into one even run per SM (per head
 // group of up to 64 heads; both groups of 128 heads walk the same tiles at
@@ -28,13 +29,25 @@
 // device.  A run's first and last sequences may be shared with its neighbours:
 // such segments go to fp32 partials that combine_kernel merges.
 //
-// Roles (10 warps): 8 softmax / accumulate warps, warpgroups with their
-// share of the heads each (thread = token for S^T, thread = latent column for O^T), a
-// TMA warp and an MMA warp.  Shared memory is a ring of 128-token x 128-byte
+// Roles (11 warps): 8 softmax warps, two warpgroups with half the heads each
+// (thread = token for S^T, thread = latent column for O^T), a TMA warp, a warp
+// for QK and one for PV.  Shared memory is a ring of 128-token x 128-byte
 // slabs (R / 128 of latents and one of rope keys per tile): a slab serves QK
-// and, as soon as its block of O^T is done, is free again, so that at 64 heads
-// (72 KB of query digits) 8 slabs suffice to run the next tile's QK ahead of
-// this tile's PV.
+// and, as soon as its block of O^T is done, is free again.
+//
+// What bounds it.  16 heads (12 slabs): HBM; 64 sequences of 1024 .. 8192
+// tokens take 43 us, 4.6 TB/s with all overheads, and a tile's 3100 cycles in
+// mid-run are the copy rate.  64 heads (72 KB of query digits leave 8 slabs):
+// the chain of a tile, 5200 cycles against 2840 of MMAs: PV's first block frees
+// a slab, the next tile's last slab is loaded into it (1300 - 1900), QK, softmax
+// (1900), PV.  128 heads, the same sequences: 128 us, 659 TFLOP/s; 32 of 4112
+// tokens 65.5 us.  At a sequence's end a run takes another 16000 cycles for
+// its output and the next query's digits.  One short sequence takes 11.5 us
+// with the merge, two launches and a tile's chain.
+// What did not help: O^T accumulated in registers per tile, one warp for QK
+// and PV, four softmax warpgroups, 48 heads per CTA (9 slabs, 138 us), a
+// reference that lags one tile behind (168 us), partials of four heads a
+// float4 (134 us).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -54,6 +67,7 @@ namespace {
 constexpr int kTileTok = 128;       // tokens per tile: MMA M
 constexpr int kMaxHeadsPerCta = 64;
 constexpr int kMaxSeqs = 65536;     // runs of sequences in the scratch
+constexpr int kMaxLen = 1 << 30;    // tokens of a sequence: token and page numbers stay in 32 bits
 constexpr int kScaleStages = 4;
 
 template <int R, int P, int HB>
@@ -92,11 +106,6 @@ struct Shape {
   static constexpr uint32_t T_COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
   static_assert(USED <= 512, "TMEM");
 };
-
-// A warp-uniform value that the compiler then knows to be one: MMA operands
-// computed from it stay in uniform registers, and branches on it do not
-// count as divergent (in either case an MMA would cost 3 times as much).
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 __device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -157,7 +166,7 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[N]) {
 }
 
 __device__ __forceinline__ bool bad_len(int len, int max_blocks) {
-  return len < 0 || len > (int64_t)max_blocks * kPageTok;
+  return len < 0 || len > kMaxLen || len > (int64_t)max_blocks * kPageTok;
 }
 
 __device__ __forceinline__ int tiles_of(int len, int max_blocks) {
@@ -468,19 +477,17 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           if (!wait(&full[c.slot], c.phase)) { ok = false; break; }
           tc_fence_after();
           const uint32_t off = (uint32_t)(c.slot * S::SLAB) >> 4;
-          {
-            if (k == 0) {
+          if (k == 0) {
 #pragma unroll
-              for (int ks = 0; ks < P / 16; ++ks) mma_bf16_ss(d, d_rope + off + ks * 2, d_qr + ks * 2, ID_QR, 1u);
-              tc_commit(&empty[c.slot]);
-            } else {
-              constexpr uint32_t kSlabQ = 2 * HB * 128 >> 4;
+            for (int ks = 0; ks < P / 16; ++ks) mma_bf16_ss(d, d_rope + off + ks * 2, d_qr + ks * 2, ID_QR, 1u);
+            tc_commit(&empty[c.slot]);
+          } else {
+            constexpr uint32_t kSlabQ = 2 * HB * 128 >> 4;
 #pragma unroll
-              for (int ks = 0; ks < 4; ++ks)
-                mma_f8_ss(d, d_slab + off + ks * 2, d_q8 + (k - 1) * kSlabQ + ks * 2, ID_QK, k > 1 || ks > 0 ? 1u : 0u);
-            }
-            if (step == NSLAB - 1) tc_commit(&s_full[n & 1]);
+            for (int ks = 0; ks < 4; ++ks)
+              mma_f8_ss(d, d_slab + off + ks * 2, d_q8 + (k - 1) * kSlabQ + ks * 2, ID_QK, k > 1 || ks > 0 ? 1u : 0u);
           }
+          if (step == NSLAB - 1) tc_commit(&s_full[n & 1]);
         }
         at.step(NSLAB);
       }
@@ -512,29 +519,26 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         int slot[NL];
 #pragma unroll
         for (int g = 0; g < NL; ++g) slot[g] = at.plus(g).slot;
-        {
 #pragma unroll
-          for (int g = 0; g < NL; ++g) {
-            const uint64_t a = d_slab + ((uint32_t)(slot[g] * S::SLAB) >> 4);
-            const uint32_t d = tmem + S::T_O + (uint32_t)(g * HB);
+        for (int g = 0; g < NL; ++g) {
+          const uint64_t a = d_slab + ((uint32_t)(slot[g] * S::SLAB) >> 4);
+          const uint32_t d = tmem + S::T_O + (uint32_t)(g * HB);
 #pragma unroll
-            for (int ks = 0; ks < kTileTok / 32; ++ks) {
-              mma_f8_ss(d, a + ks * (4096 >> 4), d_p + ks * (512 >> 4), ID_PV, first && ks == 0 ? 0u : 1u);
-              mma_f8_ss(d, a + ks * (4096 >> 4), d_p + (S::P_BYTES >> 4) + ks * (512 >> 4), ID_PV, 1u);
-            }
-            tc_commit(&empty[slot[g]]);
+          for (int ks = 0; ks < kTileTok / 32; ++ks) {
+            mma_f8_ss(d, a + ks * (4096 >> 4), d_p + ks * (512 >> 4), ID_PV, first && ks == 0 ? 0u : 1u);
+            mma_f8_ss(d, a + ks * (4096 >> 4), d_p + (S::P_BYTES >> 4) + ks * (512 >> 4), ID_PV, 1u);
           }
-          tc_commit(pv_done);
+          tc_commit(&empty[slot[g]]);
         }
+        tc_commit(pv_done);
         at.step(NSLAB);
       }
       if (!ok) raise_abort(abort, status, kStatusTimeout);
       tc_commit(&drain[1]);
       mbar_wait(&drain[1], 0, no_abort);
     }
-  } else {
-    // ------------------------------------------- softmax / accumulate warps
-    if (count > 0) {
+  } else if (count > 0) {
+    // ------------------------------------------------------- softmax warps
     const int wg = warp >> 2, quarter = warp & 3;
     const int j = quarter * 32 + lane;  // token of the tile; row of an O^T block
     const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -543,7 +547,9 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     float* mt = reinterpret_cast<float*>(smem + S::OFF_MT) + warp * HW;
     float* fh = reinterpret_cast<float*>(smem + S::OFF_FH);
     const int h0 = hg * HB;  // first head of the group
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+    };
 
     // Query digits of sequence b: a warp per head, 16 (4) latents a lane.  A
     // warpgroup loads its own heads: its warps have all read the old factors
@@ -553,79 +559,80 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       constexpr int NQ = HW / 4 < 4 ? HW / 4 : 4;  // heads whose loads are in flight together
 #pragma unroll 1
       for (int i0 = 0; i0 < HW / 4; i0 += NQ) {
-      uint32_t xs[NQ][CPL / 2];
-      uint4 rs[NQ];
+        uint32_t xs[NQ][CPL / 2];
+        uint4 rs[NQ];
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        const int h = wg * HW + quarter + 4 * (i0 + q);
-        const int64_t row = (int64_t)b * H + h0 + h;
-        rs[q] = make_uint4(0, 0, 0, 0);
+        for (int q = 0; q < NQ; ++q) {
+          const int h = wg * HW + quarter + 4 * (i0 + q);
+          const int64_t row = (int64_t)b * H + h0 + h;
+          rs[q] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < CPL / 2; ++i) xs[q][i] = 0;
-        if (h0 + h < H) {
-          if constexpr (CPL == 16) {
-            const uint4* src = reinterpret_cast<const uint4*>(q_lat + row * R + lane * 16);
-            const uint4 u = src[0], v = src[1];
-            xs[q][0] = u.x, xs[q][1] = u.y, xs[q][2] = u.z, xs[q][3] = u.w;
-            xs[q][4] = v.x, xs[q][5] = v.y, xs[q][6] = v.z, xs[q][7] = v.w;
-          } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(q_lat + row * R + lane * 4);
-            xs[q][0] = u.x, xs[q][1] = u.y;
+          for (int i = 0; i < CPL / 2; ++i) xs[q][i] = 0;
+          if (h0 + h < H) {
+            if constexpr (CPL == 16) {
+              const uint4* src = reinterpret_cast<const uint4*>(q_lat + row * R + lane * 16);
+              const uint4 u = src[0], v = src[1];
+              xs[q][0] = u.x, xs[q][1] = u.y, xs[q][2] = u.z, xs[q][3] = u.w;
+              xs[q][4] = v.x, xs[q][5] = v.y, xs[q][6] = v.z, xs[q][7] = v.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(q_lat + row * R + lane * 4);
+              xs[q][0] = u.x, xs[q][1] = u.y;
+            }
+            if (lane < P / 8) rs[q] = *reinterpret_cast<const uint4*>(q_rope + row * P + lane * 8);
           }
-          if (lane < P / 8) rs[q] = *reinterpret_cast<const uint4*>(q_rope + row * P + lane * 8);
         }
-      }
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) {
-        const int h = wg * HW + quarter + 4 * (i0 + q);
-        const uint32_t (&x)[CPL / 2] = xs[q];
-        const uint4 r = rs[q];
-        const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
-        uint32_t am = 0, rm = 0;  // magnitudes, two bf16 at once: their order is that of the bits
+        for (int q = 0; q < NQ; ++q) {
+          const int h = wg * HW + quarter + 4 * (i0 + q);
+          const uint32_t (&x)[CPL / 2] = xs[q];
+          const uint4 r = rs[q];
+          const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
+          uint32_t am = 0, rm = 0;  // magnitudes, two bf16 at once: their order is that of the bits
 #pragma unroll
-        for (int i = 0; i < CPL / 2; ++i) am = max_u16x2(am, x[i] & 0x7fff7fffu);
+          for (int i = 0; i < CPL / 2; ++i) am = max_u16x2(am, x[i] & 0x7fff7fffu);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) rm = max_u16x2(rm, rr[i] & 0x7fff7fffu);
-        const float al = __uint_as_float(max(am & 0xffff0000u, am << 16));
-        const float ar = __uint_as_float(max(rm & 0xffff0000u, rm << 16));
-        // the latents' scale; a rope part over 64 times larger sets it
-        // instead (it is divided by the same factor, in bf16, exactly)
-        const float top = redux_max(fmaxf(al, ar * 0.015625f));
-        const int e = min(100, max(-100, top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 7 : 0));
-        const float inv = exp2i(-e);
-        const uint64_t inv2 = pair(inv, inv);
-        uint32_t hi[CPL / 4], lo[CPL / 4];
+          for (int i = 0; i < 4; ++i) rm = max_u16x2(rm, rr[i] & 0x7fff7fffu);
+          const float al = __uint_as_float(max(am & 0xffff0000u, am << 16));
+          const float ar = __uint_as_float(max(rm & 0xffff0000u, rm << 16));
+          // the latents' scale; a rope part over 64 times larger sets it
+          // instead (it is divided by the same factor, in bf16, exactly)
+          const float top = redux_max(fmaxf(al, ar * 0.015625f));
+          const int e = min(100, max(-100, top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 7 : 0));
+          const float inv = exp2i(-e);
+          const uint64_t inv2 = pair(inv, inv);
+          uint32_t hi[CPL / 4], lo[CPL / 4];
 #pragma unroll
-        for (int i = 0; i < CPL / 4; ++i) {
-          uint32_t a, b2, c, d;
-          float v[4];
-          unpair(mul2(pair(bf16lo_to_f32(x[2 * i]), bf16hi_to_f32(x[2 * i])), inv2), v[0], v[1]);
-          unpair(mul2(pair(bf16lo_to_f32(x[2 * i + 1]), bf16hi_to_f32(x[2 * i + 1])), inv2), v[2], v[3]);
-          split_digits(v[0], v[1], a, b2);
-          split_digits(v[2], v[3], c, d);
-          hi[i] = a | (c << 16);
-          lo[i] = b2 | (d << 16);
+          for (int i = 0; i < CPL / 4; ++i) {
+            uint32_t a, b2, c, d;
+            float v[4];
+            unpair(mul2(pair(bf16lo_to_f32(x[2 * i]), bf16hi_to_f32(x[2 * i])), inv2), v[0], v[1]);
+            unpair(mul2(pair(bf16lo_to_f32(x[2 * i + 1]), bf16hi_to_f32(x[2 * i + 1])), inv2), v[2], v[3]);
+            split_digits(v[0], v[1], a, b2);
+            split_digits(v[2], v[3], c, d);
+            hi[i] = a | (c << 16);
+            lo[i] = b2 | (d << 16);
+          }
+          // row h (hi) and HB + h (lo) of each 128-column slab, 16-byte chunk c
+          // of a row at c ^ (row & 7)
+          const int col = lane * CPL, slab = col / 128, chunk = (col % 128) / 16, in = col % 16;
+          uint8_t* q8 = smem + S::OFF_Q8 + slab * 2 * HB * 128 + ((chunk ^ (h & 7)) * 16) + in;
+          if constexpr (CPL == 16) {
+            *reinterpret_cast<uint4*>(q8 + h * 128) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(q8 + (HB + h) * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          } else {
+            *reinterpret_cast<uint32_t*>(q8 + h * 128) = hi[0];
+            *reinterpret_cast<uint32_t*>(q8 + (HB + h) * 128) = lo[0];
+          }
+          if (lane < P / 8) {
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(bf16lo_to_f32(rr[i]) * inv, bf16hi_to_f32(rr[i]) * inv);
+            const int c = P == 64 ? (lane ^ (h & 7)) : (lane ^ ((h >> 1) & 3));
+            *reinterpret_cast<uint4*>(smem + S::OFF_QR + h * (P * 2) + c * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+          // (an infinite query would saturate to a finite one: NaN instead)
+          if (lane == 0) fh[h] = (top < INFINITY ? exp2i(e) : NAN) * scale_log2;
         }
-        // row h (hi) and HB + h (lo) of each 128-column slab, 16-byte chunk c
-        // of a row at c ^ (row & 7)
-        const int col = lane * CPL, slab = col / 128, chunk = (col % 128) / 16, in = col % 16;
-        uint8_t* q8 = smem + S::OFF_Q8 + slab * 2 * HB * 128 + ((chunk ^ (h & 7)) * 16) + in;
-        if constexpr (CPL == 16) {
-          *reinterpret_cast<uint4*>(q8 + h * 128) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(q8 + (HB + h) * 128) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        } else {
-          *reinterpret_cast<uint32_t*>(q8 + h * 128) = hi[0];
-          *reinterpret_cast<uint32_t*>(q8 + (HB + h) * 128) = lo[0];
-        }
-        if (lane < P / 8) {
-          uint32_t o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(bf16lo_to_f32(rr[i]) * inv, bf16hi_to_f32(rr[i]) * inv);
-          const int c = P == 64 ? (lane ^ (h & 7)) : (lane ^ ((h >> 1) & 3));
-          *reinterpret_cast<uint4*>(smem + S::OFF_QR + h * (P * 2) + c * 16) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
-        if (lane == 0) fh[h] = exp2i(e) * scale_log2;
-      }
       }
       fence_proxy_async_shared();
       warp_arrive(q_ready);
@@ -827,7 +834,8 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           // probability as NaN: this warpgroup clears its share of the slabs
           const uint4 z = make_uint4(0, 0, 0, 0);
           for (int g = wg; g < NL; g += NWG) {
-            uint4* r = reinterpret_cast<uint4*>(smem + S::OFF_RING + (int)(((int64_t)n * NSLAB + 1 + g) % NS) * S::SLAB + j * 128);
+            const int slot = (int)(((int64_t)n * NSLAB + 1 + g) % NS);
+            uint4* r = reinterpret_cast<uint4*>(smem + S::OFF_RING + slot * S::SLAB + j * 128);
 #pragma unroll 1
             for (int i = 0; i < 8; ++i) r[i] = z;
           }
@@ -837,7 +845,8 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         warp_arrive(p_full);
         first = false;
 #pragma unroll
-        for (int h = 0; h < HW; h += 2) unpair(fma2(pair(u[h], u[h + 1]), isig2, pair(ls[h], ls[h + 1])), ls[h], ls[h + 1]);
+        for (int h = 0; h < HW; h += 2)
+          unpair(fma2(pair(u[h], u[h + 1]), isig2, pair(ls[h], ls[h + 1])), ls[h], ls[h + 1]);
         if (n + 1 < count) w.next();
       }
       if (!seg_end) continue;
@@ -922,7 +931,6 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       ++n_seg;
     }
     if (!ok) raise_abort(abort, status, kStatusTimeout);
-    }
   }
 
   tc_fence_before();
@@ -936,7 +944,8 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
 // Sequences shared by several runs (their partials: sum_i 2^(m_i - M) O_i /
 // sum_i 2^(m_i - M) l_i), and empty ones (zero rows).  A CTA per (sequence,
 // head), its warps taking every 8th partial; with many sequences (few
-// partials each) a warp per head.
+// partials each) a warp per head.  Bound by the partials' bytes out of L2: 6 -
+// 10 us at 128 heads, under 3 at 16.
 constexpr int kCombineWarps = 8;
 
 template <int R, bool kWarpPerHead>
@@ -958,7 +967,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
     return;
   }
   if (mine.x == kSeqWhole || (kWarpPerHead && h >= H)) return;
-  const int i0 = mine.x >> 1, i1 = mine.y;
+  // (bounded, because a call that gave up leaves them unwritten)
+  const int i0 = max(0, min(mine.x >> 1, runs - 1)), i1 = min(mine.y, runs - 1);
   // partial slots: a run's first segment, then its last
   const int cta0 = h / HB * runs, hl = h % HB;
   float m = -INFINITY, l = 0.0f;
@@ -1053,8 +1063,8 @@ int launch(dsb_ctx* ctx, const void* q_lat, const void* q_rope, const void* cach
                                seq_lens, B, H, runs, softmax_scale * 1.4426950408889634f,
                                static_cast<__nv_bfloat16*>(out), ws_o, ws_ml, seq_runs, ctx->d_status));
   auto combine = [&](auto kernel, unsigned y) {
-    return launch_pdl(kernel, dim3((unsigned)B, y), kCombineWarps * 32, 0, ctx->stream, seq_runs, H, HB, runs, ws_o, ws_ml,
-                      static_cast<__nv_bfloat16*>(out));
+    return launch_pdl(kernel, dim3((unsigned)B, y), kCombineWarps * 32, 0, ctx->stream, seq_runs, H, HB, runs, ws_o,
+                      ws_ml, static_cast<__nv_bfloat16*>(out));
   };
   // a sequence has about runs / B partials
   if (B >= 32) DSB_CUDA_TRY(ctx, combine(combine_kernel<R, true>, (unsigned)((H + kCombineWarps - 1) / kCombineWarps)));
@@ -1079,7 +1089,7 @@ extern "C" int dsb_mla_decode_fp8(dsb_ctx* ctx, const void* q_lat, const void* q
   if (!cache_shape_ok(R, P))
     return fail(ctx, DSB_EUNSUPPORTED, "dsb_mla_decode_fp8: (R, P) = (%d, %d) not supported", R, P);
   if (B <= 0 || B > kMaxSeqs || H <= 0 || H > 128 || max_blocks <= 0 || n_blocks <= 0 || n_blocks >= (1 << 25) ||
-      !std::isfinite(softmax_scale))
+      (int64_t)B * max_blocks > INT32_MAX || !std::isfinite(softmax_scale))
     return fail(ctx, DSB_EINVAL, "dsb_mla_decode_fp8: bad arguments B=%d H=%d max_blocks=%d n_blocks=%lld scale=%g", B,
                 H, max_blocks, (long long)n_blocks, softmax_scale);
   if ((reinterpret_cast<uintptr_t>(q_lat) | reinterpret_cast<uintptr_t>(q_rope) | reinterpret_cast<uintptr_t>(scales) |

@@ -22,6 +22,16 @@
 // the rows that do see them.  Persistent CTAs walk the items, heavy ones
 // first within groups of heads whose keys and values stay in L2; an item's
 // prologue overlaps the last one's epilogue.
+//
+// Bound by the tensor core and, before it, by power: at 128 heads one prompt
+// of 4096 rows (causal) takes 730 us and 1024 rows behind 3000 keys 300 us,
+// 940 - 1000 TFLOP/s at 1.6 - 1.75 GHz under the 1000 W limit (cuBLAS sustains
+// 1386 there); 32 prompts of about 512 rows at 16 heads 96 us, 2.3 times the
+// time of their bytes: an item is only 1 to 4 steps long, so that its Q load,
+// first softmax and output show.  What did not help: an MMA warp for each tile
+// (15% slower: the tiles fall into step), two softmax warpgroups a tile, P
+// handed over in halves, part of the exponentials as polynomials, the next
+// item's first scores ahead of this item's output.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -157,7 +167,8 @@ __device__ __forceinline__ void store_rows(uint32_t (&w)[16], __nv_bfloat16* dst
 #pragma unroll
   for (int q = 0; q < 4; ++q)
     if (q < n_live)
-      *reinterpret_cast<uint4*>(dst + q * ld + (lane & 3) * 8) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+      *reinterpret_cast<uint4*>(dst + q * ld + (lane & 3) * 8) =
+          make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
 }
 
 template <int NOPE, int P, int VD>
@@ -233,7 +244,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = (uint32_t)uniform((int)misc[0]);
   const uint32_t smem_base = smem_u32(smem);
   const bool causal = a.causal != 0;
-  auto wait = [&](uint64_t* bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
+  };
   bool ok = true;
   // 384 threads were launched with 168 registers each; the softmax warps hold
   // a row's 128 scores: 256 * 208 + 128 * 88 = 384 * 168
@@ -296,120 +309,114 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (n_item > 0) mbar_wait(q_full, (n_item - 1) & 1u, no_abort);
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------- MMA issuer
-    // The whole warp walks and waits, one elected lane issues, operands in
-    // uniform registers (an MMA issued otherwise costs 147 cycles; so 66).
+    // One elected lane runs the role, its operands in uniform registers (an MMA
+    // issued from a lane == 0 branch costs 147 cycles; so 66 at N = 128).
     DSB_FEW_REGS;
     if (elect_one()) {
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort); };
-    constexpr uint32_t ID_QK = idesc_bf16_f32(128, 128, 0, 0), ID_PV = idesc_bf16_f32(128, VD, 0, 1);
-    const uint64_t d_q = smem_desc(smem_base + S::OFF_Q, 16, 1024, kSwizzle128B);
-    const uint64_t d_k = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
-    const uint64_t d_qr = P == 64 ? d_q : smem_desc(smem_base + S::OFF_Q, 16, 512, kSwizzle64B);
-    const uint64_t d_kr = P == 64 ? d_k : smem_desc(smem_base + S::OFF_RING, 16, 512, kSwizzle64B);
-    const uint64_t d_v = smem_desc(smem_base + S::OFF_RING, S::SLAB, 1024, kSwizzle128B);
-    Ring<NS> ring;
-    uint32_t n_item = 0, n_safe = 0;
-    uint32_t step_of[2] = {0, 0}, item_of[2] = {0, 0};  // PV steps and items of each tile
-    int k_slot[NQ], v_slot = 0;
-    // K of the next step has landed
-    auto wait_k = [&]() {
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort); };
+      constexpr uint32_t ID_QK = idesc_bf16_f32(128, 128, 0, 0), ID_PV = idesc_bf16_f32(128, VD, 0, 1);
+      const uint64_t d_q = smem_desc(smem_base + S::OFF_Q, 16, 1024, kSwizzle128B);
+      const uint64_t d_k = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
+      const uint64_t d_qr = P == 64 ? d_q : smem_desc(smem_base + S::OFF_Q, 16, 512, kSwizzle64B);
+      const uint64_t d_kr = P == 64 ? d_k : smem_desc(smem_base + S::OFF_RING, 16, 512, kSwizzle64B);
+      const uint64_t d_v = smem_desc(smem_base + S::OFF_RING, S::SLAB, 1024, kSwizzle128B);
+      Ring<NS> ring;
+      uint32_t n_item = 0, n_safe = 0;
+      uint32_t step_of[2] = {0, 0}, item_of[2] = {0, 0};  // PV steps and items of each tile
+      int k_slot[NQ], v_slot = 0;
+      // K of the next step has landed
+      auto wait_k = [&]() {
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        k_slot[i] = ring.take(1);
-        if (!wait(&full[k_slot[i]], ring.phase(k_slot[i]))) return false;
-        ring.flip(k_slot[i]);
-      }
-      tc_fence_after();
-      return true;
-    };
-    auto issue_qk = [&](int t) {
-      const uint32_t d = tmem + S::T_S + t * 128;
-      const uint32_t qo = (uint32_t)(t * NQ * S::SLAB) >> 4;
-      {
+        for (int i = 0; i < NQ; ++i) {
+          k_slot[i] = ring.take(1);
+          if (!wait(&full[k_slot[i]], ring.phase(k_slot[i]))) return false;
+          ring.flip(k_slot[i]);
+        }
+        tc_fence_after();
+        return true;
+      };
+      auto issue_qk = [&](int t) {
+        const uint32_t d = tmem + S::T_S + t * 128;
+        const uint32_t qo = (uint32_t)(t * NQ * S::SLAB) >> 4;
 #pragma unroll
         for (int i = 0; i < NN; ++i)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            mma_bf16_ss(d, d_q + qo + ((i * S::SLAB) >> 4) + ks * 2, d_k + ((uint32_t)(k_slot[i] * S::SLAB) >> 4) + ks * 2,
-                        ID_QK, i > 0 || ks > 0 ? 1u : 0u);
+            mma_bf16_ss(d, d_q + qo + ((i * S::SLAB) >> 4) + ks * 2,
+                        d_k + ((uint32_t)(k_slot[i] * S::SLAB) >> 4) + ks * 2, ID_QK, i > 0 || ks > 0 ? 1u : 0u);
 #pragma unroll
         for (int ks = 0; ks < P / 16; ++ks)
           mma_bf16_ss(d, d_qr + qo + ((NN * S::SLAB) >> 4) + ks * 2,
                       d_kr + ((uint32_t)(k_slot[NN] * S::SLAB) >> 4) + ks * 2, ID_QK, 1u);
         tc_commit(&s_full[t]);
-      }
-    };
-    auto release_k = [&]() {
-      {
+      };
+      auto release_k = [&]() {
 #pragma unroll
         for (int i = 0; i < NQ; ++i) tc_commit(&empty[k_slot[i]]);
-      }
-    };
-    for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
-      Item x;
-      bool bad;
-      if (!get_item(a, order, it, &x, &bad) || x.steps() == 0) continue;
-      const int n = x.steps();
-      ok = wait(q_full, n_item & 1u) && wait_k();
-      if (!ok) break;
-      ++n_item;
+      };
+      for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
+        Item x;
+        bool bad;
+        if (!get_item(a, order, it, &x, &bad) || x.steps() == 0) continue;
+        const int n = x.steps();
+        ok = wait(q_full, n_item & 1u) && wait_k();
+        if (!ok) break;
+        ++n_item;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (x.n[t] > 0) issue_qk(t);
-      release_k();
-      if (n == 1) tc_commit(q_empty);
-      const int full_keys = x.common(causal);
-      for (int s = 0; ok && s < n; ++s) {
-        // V of this step
-        v_slot = ring.take(NV);
+        for (int t = 0; t < 2; ++t)
+          if (x.n[t] > 0) issue_qk(t);
+        release_k();
+        if (n == 1) tc_commit(q_empty);
+        const int full_keys = x.common(causal);
+        for (int s = 0; ok && s < n; ++s) {
+          // V of this step
+          v_slot = ring.take(NV);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          ok = ok && wait(&full[v_slot + i], ring.phase(v_slot + i));
-          ring.flip(v_slot + i);
-        }
-        if (ok && (s + 1) * kRows > full_keys) {  // its masked values have been seen to
-          ok = wait(&v_safe[n_safe & 3u], (n_safe >> 2) & 1u);
-          ++n_safe;
-        }
-        const int vs = v_slot;
-        const bool more = s + 1 < n;
+          for (int i = 0; i < NV; ++i) {
+            ok = ok && wait(&full[v_slot + i], ring.phase(v_slot + i));
+            ring.flip(v_slot + i);
+          }
+          if (ok && (s + 1) * kRows > full_keys) {  // its masked values have been seen to
+            ok = wait(&v_safe[n_safe & 3u], (n_safe >> 2) & 1u);
+            ++n_safe;
+          }
+          const int vs = v_slot;
+          const bool more = s + 1 < n;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (ok && s < x.n[t]) {
-            if (s == 0 && item_of[t]++ > 0) ok = wait(&o_free[t], (item_of[t] - 2) & 1u);
-            ok = ok && wait(&p_full[t], step_of[t] & 1u);
-            if (!ok) break;
-            ++step_of[t];
-            tc_fence_after();
-            const uint32_t d = tmem + S::T_O + t * 128, p = tmem + S::T_S + t * 128;
-            const uint64_t v = d_v + ((uint32_t)(vs * S::SLAB) >> 4);
-            {
+          for (int t = 0; t < 2; ++t) {
+            if (ok && s < x.n[t]) {
+              if (s == 0 && item_of[t]++ > 0) ok = wait(&o_free[t], (item_of[t] - 2) & 1u);
+              ok = ok && wait(&p_full[t], step_of[t] & 1u);
+              if (!ok) break;
+              ++step_of[t];
+              tc_fence_after();
+              const uint32_t d = tmem + S::T_O + t * 128, p = tmem + S::T_S + t * 128;
+              const uint64_t v = d_v + ((uint32_t)(vs * S::SLAB) >> 4);
 #pragma unroll
               for (int ks = 0; ks < kRows / 16; ++ks)
                 mma_bf16_ts(d, p + ks * 8, v + ks * (2048 >> 4), ID_PV, s > 0 || ks > 0 ? 1u : 0u);
               tc_commit(&pv_done[t]);
             }
-          }
-          if (t == 1) {
+            if (t == 1) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) tc_commit(&empty[vs + i]);
-          }
-          if (ok && more) {
-            // the next scores of this tile, while the other tile's softmax runs
-            if (t == 0) ok = wait_k();
-            if (ok && s + 1 < x.n[t]) issue_qk(t);
-            if (ok && t == 1) {
-              release_k();
-              if (s + 2 == n) tc_commit(q_empty);
+              for (int i = 0; i < NV; ++i) tc_commit(&empty[vs + i]);
+            }
+            if (ok && more) {
+              // the next scores of this tile, while the other tile's softmax runs
+              if (t == 0) ok = wait_k();
+              if (ok && s + 1 < x.n[t]) issue_qk(t);
+              if (ok && t == 1) {
+                release_k();
+                if (s + 2 == n) tc_commit(q_empty);
+              }
             }
           }
         }
       }
-    }
-    if (!ok) raise_abort(abort, status, kStatusTimeout);
-    // every issued MMA must finish before TMEM and shared memory are released
-    tc_commit(drain);
-    mbar_wait(drain, 0, no_abort);
+      if (!ok) raise_abort(abort, status, kStatusTimeout);
+      // every issued MMA must finish before TMEM and shared memory are released
+      tc_commit(drain);
+      mbar_wait(drain, 0, no_abort);
     }
   } else if (warp >= kScanWarp) {
     // ------------------------------------- masked values (each warp one half)
@@ -598,7 +605,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       // -------------------------------------------------------------- result
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      if (live && a.lse != nullptr) a.lse[row * a.H + x.h] = l > 0.0f ? m * 0.6931471805599453f + logf(l) : l == 0.0f ? -INFINITY : l;
+      if (live && a.lse != nullptr)
+        a.lse[row * a.H + x.h] = l > 0.0f ? m * 0.6931471805599453f + logf(l) : l == 0.0f ? -INFINITY : l;
       __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.out) + row * a.ld_out + (int64_t)x.h * VD;
       const uint32_t* word = reinterpret_cast<const uint32_t*>(smem + S::OFF_BAD + (n_item % 3) * S::BAD_BYTES);
       const uint32_t* any = word + VD;
@@ -671,7 +679,9 @@ int launch(dsb_ctx* ctx, const dsb_mla_prefill_args& a) {
     const bool rope = i == 1 || i == 3;
     const int64_t heads = i == 3 ? 1 : a.H;
     const int box = rope ? P : 64;
-    if (int rc = make_tmap_2d(ctx, &m[i], t[i].p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+    // no key is loaded where there is none: any valid address will do
+    const void* base = i >= 2 && a.Tk == 0 ? a.out : t[i].p;
+    if (int rc = make_tmap_2d(ctx, &m[i], base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                               (uint64_t)((heads - 1) * t[i].hd + t[i].dim), (uint64_t)std::max(1, t[i].rows),
                               (uint64_t)t[i].ld * 2, (uint32_t)box, kRows,
                               box == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
@@ -680,7 +690,8 @@ int launch(dsb_ctx* ctx, const dsb_mla_prefill_args& a) {
   }
   Order o;
   o.pairs = a.B * a.H;
-  o.blocks = (int)(((int64_t)a.max_q + 2 * kRows - 1) / (2 * kRows));
+  // (one with max_q = 0 too: the lengths are checked)
+  o.blocks = std::max(1, (int)(((int64_t)a.max_q + 2 * kRows - 1) / (2 * kRows)));
   // heads per group: two items for every SM, so that a group's keys and
   // values are read from HBM once and from L2 by the other blocks
   o.group = std::min(o.pairs, std::max(1, (2 * ctx->sm_count + o.blocks - 1) / o.blocks));
@@ -708,8 +719,10 @@ extern "C" int dsb_mla_prefill(dsb_ctx* ctx, const dsb_mla_prefill_args* args) {
   if (ctx == nullptr) return DSB_EINVAL;
   if (args == nullptr) return fail(ctx, DSB_EINVAL, "dsb_mla_prefill: null arguments");
   const dsb_mla_prefill_args& a = *args;
-  if (a.q_nope == nullptr || a.q_rope == nullptr || a.k_nope == nullptr || a.k_rope == nullptr || a.v == nullptr ||
-      a.cu_q == nullptr || a.cu_k == nullptr || a.out == nullptr)
+  // (an empty tensor may come without memory)
+  if (a.cu_q == nullptr || a.cu_k == nullptr ||
+      (a.Tq != 0 && (a.q_nope == nullptr || a.q_rope == nullptr || a.out == nullptr)) ||
+      (a.Tk != 0 && (a.k_nope == nullptr || a.k_rope == nullptr || a.v == nullptr)))
     return fail(ctx, DSB_EINVAL, "dsb_mla_prefill: null pointer argument");
   const bool big = a.nope == 128 && a.P == 64 && a.vd == 128, small = a.nope == 64 && a.P == 32 && a.vd == 64;
   if (!big && !small)
@@ -733,7 +746,7 @@ extern "C" int dsb_mla_prefill(dsb_ctx* ctx, const dsb_mla_prefill_args* args) {
        reinterpret_cast<uintptr_t>(a.k_nope) | reinterpret_cast<uintptr_t>(a.k_rope) |
        reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.out)) & 15u)
     return fail(ctx, DSB_EINVAL, "dsb_mla_prefill: pointers must be 16-byte aligned");
-  if (a.Tq == 0 || a.max_q == 0) return DSB_OK;
+  if (a.Tq == 0) return DSB_OK;
   DeviceScope scope(ctx->device);
   if (!scope.ok) return fail(ctx, DSB_ECUDA, "dsb_mla_prefill: cudaSetDevice(%d) failed", ctx->device);
   return big ? launch<128, 64, 128>(ctx, a) : launch<64, 32, 64>(ctx, a);

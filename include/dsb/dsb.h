@@ -383,10 +383,13 @@ DSB_API int dsb_kv_norm_rope_append_fp8(dsb_ctx* ctx, const float* kv_a, int64_t
  * over the seq_lens[b] cached tokens of sequence b (a length of 0 gives a zero
  * row).  seq_lens is a DEVICE int32 [B]: the kernel splits the work itself, so
  * a captured call may be replayed with other lengths.  Cache rows past a
- * length are not used, whatever they hold.  Scratch comes from the context
- * (39 MB, allocated by the first call): calls of one context must not overlap
- * on the GPU.  H <= 128; q_lat, q_rope, out_lat bf16 as in dsb_mla_decode,
- * 16-byte aligned; n_blocks <= 2^25 - 1. */
+ * length are not used, whatever they hold.  Scales must be positive; a token
+ * whose scale is 2^-40 of its sequence's largest or less may count as a zero
+ * row, one of scale 0 (a row never written) counts as 2^-100.  Scratch comes
+ * from the context (39 MB, allocated by the first call): calls of one context
+ * must not overlap on the GPU.  H <= 128, B <= 65536, B * max_blocks < 2^31,
+ * lengths <= 2^30, n_blocks < 2^25; q_lat, q_rope, out_lat bf16 as in
+ * dsb_mla_decode, 16-byte aligned; so are cache and scales. */
 DSB_API int dsb_mla_decode_fp8(dsb_ctx* ctx, const void* q_lat, const void* q_rope, const void* cache,
                                const float* scales, int64_t n_blocks, const int32_t* block_table, int max_blocks,
                                const int32_t* seq_lens, int B, int H, int R, int P, float softmax_scale,
@@ -397,8 +400,9 @@ DSB_API int dsb_mla_decode_fp8(dsb_ctx* ctx, const void* q_lat, const void* q_ro
  * Sequence b's first cu_seqlens[b+1] - cu_seqlens[b] tokens go to rows
  * cu_seqlens[b] .. of latent [T, R] (row pitch ld_lat) and k_rope [T, P] (row
  * pitch ld_rope); either may be NULL.  cu_seqlens device int32 [B + 1],
- * ascending from 0; rows at or past cu_seqlens[B] (T is the buffers' row
- * count) are left as they were.  Exact.  Outputs 16-byte aligned, pitches
+ * ascending from 0 to at most T, the buffers' row count (more sets the status
+ * word; the rows that fit are read); rows at or past cu_seqlens[B] are left as
+ * they were.  Exact.  Outputs 16-byte aligned, pitches
  * multiples of 8. */
 DSB_API int dsb_mla_cache_read_fp8(dsb_ctx* ctx, const void* cache, const float* scales, int64_t n_blocks,
                                    const int32_t* block_table, int max_blocks, const int32_t* cu_seqlens, int B,
@@ -419,10 +423,11 @@ DSB_API int dsb_mla_cache_read_fp8(dsb_ctx* ctx, const void* cache, const float*
  * sizes the grid, and rows beyond it set the status word (dsb_sync returns
  * DSB_EINVAL) and are left as they were.
  * All tensors bf16 with a token pitch ld_* and, where there are heads, a head
- * pitch hd_* in elements, multiples of 8 (so k_nope and v may be the two
- * halves of one kv_b projection, q_nope the front of each head of q);
- * pointers 16-byte aligned.  out [Tq, ld_out], head h at column h * vd; lse
- * fp32 [Tq, H] or NULL.  Supported (nope, P, vd): (128, 64, 128), (64, 32, 64). */
+ * pitch hd_* in elements, multiples of 8, a token's heads within its pitch (so
+ * k_nope and v may be the two halves of one kv_b projection, q_nope the front
+ * of each head of q); pointers 16-byte aligned (NULL where Tq or Tk is 0).
+ * out [Tq, ld_out], head h at column h * vd; lse fp32 [Tq, H] or NULL.
+ * B <= 65535, H <= 4096, Tk < 2^28, B * H * ceil(max_q / 256) < 2^30.  Supported (nope, P, vd): (128, 64, 128), (64, 32, 64). */
 typedef struct dsb_mla_prefill_args {
   const void* q_nope;
   int64_t ld_q_nope, hd_q_nope;

@@ -370,6 +370,37 @@ def test_decode_bad_lengths_and_pages_are_reported(gpu_ctx):
             check_decode(out[b:b + 1], q_lat[b:b + 1], q_rope[b:b + 1], cache, scales, table[b:b + 1], [lens[b]], scale)
 
 
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_decode_non_finite_query_stays_in_its_head(gpu_ctx, value):
+    """Its scores are infinite or NaN, so its softmax is NaN; the other heads and sequences keep their bounds.  (Not
+    their bits: next to a NaN the tile's maxima come from the fp32 path, and a reference that differs in its last
+    bits moves the digits' roundings, which the bound counts.)"""
+    lens = [300, 200]
+    q_lat, q_rope, cache, scales, table, scale = decode_inputs(lens, 16, BIG, seed=19)
+    bad_lat, bad_rope = q_lat.clone(), q_rope.clone()
+    bad_lat[0, 3, 100] = value
+    bad_rope[1, 9, 5] = value
+    out = run_decode(gpu_ctx, bad_lat, bad_rope, cache, scales, table, lens, scale)
+    clean = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, lens, scale)
+    gpu_ctx.sync()
+    assert out[0, 3].isnan().all() and out[1, 9].isnan().all()
+    out[0, 3], out[1, 9] = clean[0, 3], clean[1, 9]
+    check_decode(out, q_lat, q_rope, cache, scales, table, lens, scale)
+
+
+def test_decode_length_beyond_32_bit_positions_is_reported(gpu_ctx):
+    """A table of 2^24 + 1 pages would hold it; positions past 2^30 are refused instead of wrapping."""
+    import torch
+
+    q_lat, q_rope, cache, scales, _, scale = decode_inputs([64], 16, SMALL, seed=18)
+    table = torch.zeros(1, (1 << 24) + 1, dtype=torch.int32, device="cuda")
+    out = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, [(1 << 30) + 1], scale)
+    with pytest.raises(DsbError) as e:
+        gpu_ctx.sync()
+    assert e.value.code == DSB_EINVAL
+    assert (out == 0).all()
+
+
 # -------------------------------------------------------------------- read
 
 
@@ -428,7 +459,32 @@ def test_read_bad_pages_are_reported(gpu_ctx):
         assert (lat[64:70] == 7.0).all() if cu[1] == 70 else (lat[138:145] == 7.0).all()
 
 
+def test_read_more_rows_than_the_buffers_hold_is_reported(gpu_ctx):
+    import torch
+
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    cache, scales = ref.make_cache(2, 128, 32, seed=4)
+    lat = torch.full((90, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    rope = torch.full((90, 32), 7.0, dtype=torch.bfloat16, device="cuda")
+    gpu_ctx.mla_cache_read_fp8(cache, scales, table, torch.tensor([0, 81], dtype=torch.int32, device="cuda"), lat[:80],
+                               rope[:80])
+    with pytest.raises(DsbError) as e:
+        gpu_ctx.sync()
+    assert e.value.code == DSB_EINVAL
+    want = ref.rows64(cache, scales, table, 0, 80, 128)
+    assert torch.equal(lat[:80].double(), want[0]) and torch.equal(rope[:80].double(), want[1])
+    assert (lat[80:] == 7.0).all() and (rope[80:] == 7.0).all()
+
+
 # ---------------------------------------------------------------- refusals
+
+
+def test_decode_table_past_32_bits_is_refused(gpu_ctx):
+    """65536 sequences of 32768 pages: an index into the table would not fit an int."""
+    d = {k: 16 for k in ("q_lat", "q_rope", "cache", "scales", "table", "lens", "out")}
+    args = (gpu_ctx.h, d["q_lat"], d["q_rope"], d["cache"], d["scales"], 1, d["table"], 1 << 15, d["lens"], 1 << 16, 16,
+            512, 64, 0.1, d["out"])
+    assert gpu_ctx._l.dsb_mla_decode_fp8(*args) == DSB_EINVAL
 
 
 def test_refusals(gpu_ctx):
@@ -463,7 +519,7 @@ def test_refusals(gpu_ctx):
              + [(DSB_EINVAL, "scale", float("nan")), (DSB_EINVAL, "scale", float("inf")), (DSB_UNSUP, "R", 256),
                 (DSB_UNSUP, "P", 32), (DSB_EINVAL, "H", 0), (DSB_EINVAL, "H", 129), (DSB_EINVAL, "B", 0),
                 (DSB_EINVAL, "max_blocks", 0), (DSB_EINVAL, "n_blocks", 0), (DSB_EINVAL, "n_blocks", 1 << 25),
-                (DSB_EINVAL, "out", p(out) + 2), (DSB_EINVAL, "q_lat", p(q_lat) + 8), (DSB_EINVAL, "cache", p(cache) + 1)]),
+                (DSB_EINVAL, "B", 65537), (DSB_EINVAL, "out", p(out) + 2), (DSB_EINVAL, "q_lat", p(q_lat) + 8), (DSB_EINVAL, "cache", p(cache) + 1)]),
             (l.dsb_kv_norm_rope_append_fp8, app,
              [(DSB_EINVAL, k, None) for k in ("ctx", "kv", "w", "q", "pos", "table", "cache", "scales", "q_rope")]
              + [(DSB_UNSUP, "R", 256), (DSB_UNSUP, "P", 128), (DSB_EINVAL, "nope", 100), (DSB_EINVAL, "nope", -8),

@@ -207,6 +207,32 @@ def test_max_q_too_small_is_reported(gpu_ctx):
     assert e.value.code == DSB_EINVAL
 
 
+def test_max_q_of_zero_is_reported(gpu_ctx):
+    lq = [100, 3]
+    x = inputs(lq, lq, 2, BIG, seed=13)
+    run(gpu_ctx, x, lq, lq, max_q=0)
+    with pytest.raises(DsbError) as e:
+        gpu_ctx.sync()
+    assert e.value.code == DSB_EINVAL
+    run(gpu_ctx, x, [0, 0], lq, max_q=0)
+    gpu_ctx.sync()
+
+
+def test_no_keys_and_no_queries_at_all(gpu_ctx):
+    """Tensors without memory: zero rows and lse = -inf, or nothing to do."""
+    import torch
+
+    x = inputs([5, 0], [0, 0], 2, BIG, seed=14)
+    x = (*x[:2], x[2][:0], x[3][:0], x[4][:0], x[5])
+    out, lse = run(gpu_ctx, x, [5, 0], [0, 0])
+    gpu_ctx.sync()
+    assert (out == 0).all() and torch.isneginf(lse).all() and out.shape[0] == 5
+    x = inputs([0, 0], [5, 200], 2, BIG, seed=15)
+    out, _ = run(gpu_ctx, x, [0, 0], [5, 200])
+    gpu_ctx.sync()
+    assert out.shape[0] == 0
+
+
 def test_captured_and_replayed(gpu_ctx):
     import torch
 
