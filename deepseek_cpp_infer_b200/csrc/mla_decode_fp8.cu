@@ -47,7 +47,10 @@
 // What did not help: O^T accumulated in registers per tile, one warp for QK
 // and PV, four softmax warpgroups, 48 heads per CTA (9 slabs, 138 us), a
 // reference that lags one tile behind (168 us), partials of four heads a
-// float4 (134 us).
+// float4 (134 us).  At 64 heads the softmax warps use all 168 registers that
+// three warps a partition leave: more loads in flight for the query's digits
+// spill, and any spill beside 228 KB of shared memory costs 5% or more
+// (setmaxnreg with a twelfth warp: 139 us).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -178,6 +181,7 @@ struct Walk {
   const int32_t* lens;
   int B, max_blocks;
   int b, tile, ntile, len;
+  int len_ahead;  // the next sequence's, read long before it is needed
   __device__ void start(const int32_t* l, int B_, int mb, int b_, int tile_) {
     lens = l;
     B = B_;
@@ -185,6 +189,7 @@ struct Walk {
     b = b_;
     tile = tile_;
     len = lens[b];
+    len_ahead = b + 1 < B ? lens[b + 1] : 1;
     ntile = tiles_of(len, max_blocks);
   }
   __device__ void next() {  // only called while tiles are left
@@ -192,7 +197,8 @@ struct Walk {
     tile = 0;
     do {
       ++b;
-      len = b < B ? lens[b] : 1;
+      len = len_ahead;
+      len_ahead = b + 1 < B ? lens[b + 1] : 1;
       ntile = tiles_of(len, max_blocks);
     } while (ntile == 0);
   }
@@ -901,18 +907,29 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           const bool s1 = lane & 1, s2 = lane & 2;
           const int mine = (s1 ? 2 : 0) + (s2 ? 1 : 0);  // of each four heads
           __nv_bfloat16* dst = out + ((int64_t)b_now * H + hb + mine) * R + g * 128 + (j & ~3);
+          // (one exchange for all heads, then the other: their latencies overlap)
+          uint32_t x[HW / 4], y[HW / 4];
 #pragma unroll
           for (int h = 0; h < HW; h += 4) {
             const float4 il = *reinterpret_cast<const float4*>(mt + h);
-            const uint32_t w01 = pack_bf16x2(__uint_as_float(o[h]) * il.x, __uint_as_float(o[h + 1]) * il.y);
-            const uint32_t w23 = pack_bf16x2(__uint_as_float(o[h + 2]) * il.z, __uint_as_float(o[h + 3]) * il.w);
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, s1 ? w01 : w23, 1);
-            const uint32_t a = s1 ? got : w01, c = s1 ? w23 : got;  // two heads of latents j & ~1 and j | 1
-            const uint32_t x = __byte_perm(a, c, 0x5410), y = __byte_perm(a, c, 0x7632);
-            const uint32_t far = __shfl_xor_sync(0xffffffffu, s2 ? x : y, 2);
-            if (hb + h + mine < H)
-              *reinterpret_cast<uint2*>(dst + h * R) = s2 ? make_uint2(far, y) : make_uint2(x, far);
+            x[h / 4] = pack_bf16x2(__uint_as_float(o[h]) * il.x, __uint_as_float(o[h + 1]) * il.y);
+            y[h / 4] = pack_bf16x2(__uint_as_float(o[h + 2]) * il.z, __uint_as_float(o[h + 3]) * il.w);
           }
+          uint32_t got[HW / 4];
+#pragma unroll
+          for (int i = 0; i < HW / 4; ++i) got[i] = __shfl_xor_sync(0xffffffffu, s1 ? x[i] : y[i], 1);
+#pragma unroll
+          for (int i = 0; i < HW / 4; ++i) {  // two heads of latents j & ~1 and j | 1
+            const uint32_t a = s1 ? got[i] : x[i], c = s1 ? y[i] : got[i];
+            x[i] = __byte_perm(a, c, 0x5410);
+            y[i] = __byte_perm(a, c, 0x7632);
+          }
+#pragma unroll
+          for (int i = 0; i < HW / 4; ++i) got[i] = __shfl_xor_sync(0xffffffffu, s2 ? x[i] : y[i], 2);
+#pragma unroll
+          for (int i = 0; i < HW / 4; ++i)
+            if (hb + 4 * i + mine < H)
+              *reinterpret_cast<uint2*>(dst + 4 * i * R) = s2 ? make_uint2(got[i], y[i]) : make_uint2(x[i], got[i]);
         } else {
           float* dst = ws_o + (slot * HB + wg * HW) * R + g * 128 + j;
 #pragma unroll
