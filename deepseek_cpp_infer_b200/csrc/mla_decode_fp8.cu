@@ -84,7 +84,6 @@ struct Shape {
   static constexpr int SLAB = kTileTok * 128;        // bytes
   static constexpr int NS = HB == 16 ? 12 : HB == 32 || NL == 1 ? 10 : 8;  // ring slots: what fits
   static_assert(NS >= NSLAB + 1, "ring");
-  static constexpr bool PREFETCH = NS < 2 * NSLAB;
   static constexpr int Q8_BYTES = 2 * HB * R;        // [slab][hi heads | lo heads][128 B], SW128
   static constexpr int QR_BYTES = HB * P * 2;        // [head][P bf16], SW128 (P = 64) or SW64
   static constexpr int P_BYTES = HB * kTileTok;      // one digit of the probabilities
@@ -147,16 +146,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                    smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
-// Bring bytes (address and size multiples of 16) or a box into L2 ahead of their load.
-__device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y)
                : "memory");
 }
 
@@ -376,13 +365,6 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       bool ok = true;
       for (int n = 0; ok && n < count; ++n) {
         if (n > 0) w.next();
-        if ((n == 0 || w.tile == 0) && w.ntile - w.tile < count - n && w.b + 1 < B && elect_one()) {
-          // the next sequence's queries into L2
-          const int64_t row = (int64_t)(w.b + 1) * H + hg * HB;
-          const int rows = min(HB, H - hg * HB);
-          prefetch_l2(q_lat + row * R, rows * R * 2);
-          prefetch_l2(q_rope + row * P, rows * P * 2);
-        }
         if (at == 32 || w.tile == 0) {
           const int p = w.tile * 2 + lane;
           pages = 0;
@@ -411,19 +393,6 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
                       kPageTok * 4, &sc_full[sc]);
         }
         ++nsc;
-        if (S::PREFETCH && at + 2 < 32) {
-          // the ring holds less than two tiles: the tile after next into L2
-          const int p0 = __shfl_sync(0xffffffffu, pages, at + 2), p1 = __shfl_sync(0xffffffffu, pages, at + 3);
-          const int left = w.len - (w.tile + 2) * kTileTok;
-          if (left > 0 && elect_one()) {
-#pragma unroll 1
-            for (int k = 0; k < NSLAB; ++k) {
-              tma_prefetch_2d(k == 0 ? &map_rope : &map_lat, k == 0 ? R : (k - 1) * 128, p0 * kPageTok);
-              if (left > kPageTok)
-                tma_prefetch_2d(k == 0 ? &map_rope : &map_lat, k == 0 ? R : (k - 1) * 128, p1 * kPageTok);
-            }
-          }
-        }
 #pragma unroll 1
         for (int k = 0; k < NSLAB; ++k, ++it) {
           const int slot = at_slab.slot;
