@@ -36,21 +36,22 @@
 // and, as soon as its block of O^T is done, is free again.
 //
 // What bounds it.  16 heads (12 slabs): HBM; 64 sequences of 1024 .. 8192
-// tokens take 43 us, 4.6 TB/s with all overheads, and a tile's 3100 cycles in
+// tokens take 41 us, 4.8 TB/s with all overheads, and a tile's 3100 cycles in
 // mid-run are the copy rate.  64 heads (72 KB of query digits leave 8 slabs):
-// the chain of a tile, 5200 cycles against 2840 of MMAs: PV's first block frees
-// a slab, the next tile's last slab is loaded into it (1300 - 1900), QK, softmax
-// (1900), PV.  128 heads, the same sequences: 128 us, 659 TFLOP/s; 32 of 4112
-// tokens 65.5 us.  At a sequence's end a run takes another 16000 cycles for
-// its output and the next query's digits.  One short sequence takes 11.5 us
-// with the merge, two launches and a tile's chain.
+// the chain of a tile, about 5000 cycles against 2840 of MMAs: PV's first block
+// frees a slab, the next tile's last slab is loaded into it (1300 - 1900), QK,
+// softmax (1900), PV.  128 heads, the same sequences: 121 us, 697 TFLOP/s; 32 of
+// 4112 tokens 65 us; 3 of 60000 .. 131072 tokens 107 us.  At a sequence's end a
+// run takes another 14000 cycles for its output and the next query's digits.
+// One short sequence takes 11.5 us with the merge, two launches and a tile's
+// chain.
 // What did not help: O^T accumulated in registers per tile, one warp for QK
 // and PV, four softmax warpgroups, 48 heads per CTA (9 slabs, 138 us), a
 // reference that lags one tile behind (168 us), partials of four heads a
 // float4 (134 us).  At 64 heads the softmax warps use all 168 registers that
 // three warps a partition leave: more loads in flight for the query's digits
 // spill, and any spill beside 228 KB of shared memory costs 5% or more
-// (setmaxnreg with a twelfth warp: 139 us).
+// (setmaxnreg with a twelfth warp: 139 us); tiles prefetched into L2 (127 us).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -928,42 +929,92 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
 }
 
 // Sequences shared by several runs (their partials: sum_i 2^(m_i - M) O_i /
-// sum_i 2^(m_i - M) l_i), and empty ones (zero rows).  A CTA per (sequence,
-// head), its warps taking every 8th partial; with many sequences (few
-// partials each) a warp per head.  Bound by the partials' bytes out of L2: 6 -
-// 10 us at 128 heads, under 3 at 16.
+// sum_i 2^(m_i - M) l_i), and empty ones (zero rows).  Many sequences have few
+// partials each (about runs / B): a warp takes 128 V columns of a head and reads
+// them in turn.  Few sequences have many: a CTA takes a head, its warps every
+// 8th partial.
+// Bound by latency for small batches: with V = 1 a CTA (128 threads, 48
+// registers, no shared memory) is resident beside a decode CTA before that ends
+// (32 sequences x 16 heads 16.4 us with the decode kernel, 64 x 16 40.9; whole
+// heads 18.1, 42.6).  Bound by the partials' bytes out of L2 for large ones, where
+// so many CTAs cost more (64 x 64 75.1 against 77.4 us, 74 x 128 whole sequences
+// 15.5 against 24.0).  Without the merge those four take 12.5, 37.7, 69.8, 13.4.
 constexpr int kCombineWarps = 8;
+constexpr int kFewFrom = 32;         // sequences
+constexpr int kSplitRows = 2048;     // sequences x heads up to which V = 1
 
-template <int R, bool kWarpPerHead>
+__device__ __forceinline__ void store_bf16x4(__nv_bfloat16* dst, const float4& v, float f) {
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
+}
+
+template <int R, int V>
+__global__ void __launch_bounds__(V == 1 ? 128 : 256, V == 1 ? 10 : 4)
+    combine_few_kernel(const int2* __restrict__ seq_runs, int H, int HB, int runs, const float* __restrict__ ws_o,
+                       const float2* __restrict__ ws_ml, __nv_bfloat16* __restrict__ out) {
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr int kPerHead = R / 128 / V, kWarps = V == 1 ? 4 : 8;  // warps
+  const int warp = (int)warp_id(), lane = (int)lane_id();
+  const int b = blockIdx.x, h = blockIdx.y * (kWarps / kPerHead) + warp / kPerHead;
+  const int col = (warp % kPerHead) * 128 * V + lane * 4;
+  const int2 mine = seq_runs[b];
+  if (mine.x == kSeqWhole || h >= H) return;
+  float4 o[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -INFINITY, l = 1.0f;
+  if (mine.x != kSeqEmpty) {
+    // (bounded, because a call that gave up leaves them unwritten)
+    const int i0 = max(0, min(mine.x >> 1, runs - 1)), i1 = min(mine.y, runs - 1);
+    // partial slots: the last segment of the first run, the first of the others
+    const int cta0 = h / HB * runs, hl = h % HB;
+    l = 0.0f;
+#pragma unroll 4
+    for (int i = i0; i <= i1; ++i) {
+      const int64_t s = (int64_t)((cta0 + i) * 2 + (i == i0 ? mine.x & 1 : 0)) * HB + hl;
+      const float2 ml = ws_ml[s];
+      const float mn = fmaxf(m, ml.x), a = fast_exp2(m - mn), c = fast_exp2(ml.x - mn);
+      m = mn;
+      l = l * a + ml.y * c;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float4 x = *reinterpret_cast<const float4*>(ws_o + s * R + col + v * 128);
+        o[v].x = o[v].x * a + x.x * c;
+        o[v].y = o[v].y * a + x.y * c;
+        o[v].z = o[v].z * a + x.z * c;
+        o[v].w = o[v].w * a + x.w * c;
+      }
+    }
+  }
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int v = 0; v < V; ++v) store_bf16x4(out + ((int64_t)b * H + h) * R + col + v * 128, o[v], inv);
+}
+
+template <int R>
 __global__ void __launch_bounds__(kCombineWarps * 32)
-    combine_kernel(const int2* __restrict__ seq_runs, int H, int HB, int runs,
-                   const float* __restrict__ ws_o, const float2* __restrict__ ws_ml, __nv_bfloat16* __restrict__ out) {
+    combine_many_kernel(const int2* __restrict__ seq_runs, int H, int HB, int runs, const float* __restrict__ ws_o,
+                        const float2* __restrict__ ws_ml, __nv_bfloat16* __restrict__ out) {
   pdl_wait();
   pdl_launch_dependents();
   constexpr int V = R / 128;  // float4 per lane
   const int warp = (int)warp_id(), lane = (int)lane_id();
-  const int b = blockIdx.x, h = kWarpPerHead ? blockIdx.y * kCombineWarps + warp : blockIdx.y;
+  const int b = blockIdx.x, h = blockIdx.y;
   const int2 mine = seq_runs[b];
+  if (mine.x == kSeqWhole) return;
   __nv_bfloat16* dst = out + ((int64_t)b * H + h) * R + lane * 4;
-  if (mine.x == kSeqEmpty) {
-    if (h < H && (kWarpPerHead || warp == 0)) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) *reinterpret_cast<uint2*>(dst + v * 128) = make_uint2(0, 0);
-    }
-    return;
-  }
-  if (mine.x == kSeqWhole || (kWarpPerHead && h >= H)) return;
-  // (bounded, because a call that gave up leaves them unwritten)
-  const int i0 = max(0, min(mine.x >> 1, runs - 1)), i1 = min(mine.y, runs - 1);
-  // partial slots: a run's first segment, then its last
-  const int cta0 = h / HB * runs, hl = h % HB;
   float m = -INFINITY, l = 0.0f;
   float4 o[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  constexpr int kStep = kWarpPerHead ? 1 : kCombineWarps;
+  if (mine.x == kSeqEmpty) {
+    if (warp < V) store_bf16x4(dst + warp * 128, o[0], 1.0f);
+    return;
+  }
+  const int i0 = max(0, min(mine.x >> 1, runs - 1)), i1 = min(mine.y, runs - 1);
+  const int cta0 = h / HB * runs, hl = h % HB;
 #pragma unroll 4
-  for (int i = i0 + (kWarpPerHead ? 0 : warp); i <= i1; i += kStep) {
+  for (int i = i0 + warp; i <= i1; i += kCombineWarps) {
     const int64_t s = (int64_t)((cta0 + i) * 2 + (i == i0 ? mine.x & 1 : 0)) * HB + hl;
     const float2 ml = ws_ml[s];
     const float mn = fmaxf(m, ml.x), a = fast_exp2(m - mn), c = fast_exp2(ml.x - mn);
@@ -978,40 +1029,30 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
       o[v].w = o[v].w * a + x.w * c;
     }
   }
-  if constexpr (!kWarpPerHead) {
-    __shared__ float sm[kCombineWarps], sl[kCombineWarps];
-    __shared__ float4 so[kCombineWarps][R / 4];
-    if (lane == 0) {
-      sm[warp] = m;
-      sl[warp] = l;
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) so[warp][v * 32 + lane] = o[v];
-    __syncthreads();
-    if (warp >= V) return;  // warp v merges columns [128 v, 128 v + 128)
-    float top = -INFINITY, den = 0.0f;
-    float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < kCombineWarps; ++i) top = fmaxf(top, sm[i]);
-    for (int i = 0; i < kCombineWarps; ++i) {
-      if (sm[i] == -INFINITY) continue;  // no partial
-      const float c = fast_exp2(sm[i] - top);
-      const float4 x = so[i][warp * 32 + lane];
-      den += sl[i] * c;
-      r.x += x.x * c;
-      r.y += x.y * c;
-      r.z += x.z * c;
-      r.w += x.w * c;
-    }
-    const float inv = 1.0f / den;
-    *reinterpret_cast<uint2*>(dst + warp * 128) =
-        make_uint2(pack_bf16x2(r.x * inv, r.y * inv), pack_bf16x2(r.z * inv, r.w * inv));
-  } else {
-    const float inv = 1.0f / l;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      *reinterpret_cast<uint2*>(dst + v * 128) =
-          make_uint2(pack_bf16x2(o[v].x * inv, o[v].y * inv), pack_bf16x2(o[v].z * inv, o[v].w * inv));
+  __shared__ float sm[kCombineWarps], sl[kCombineWarps];
+  __shared__ float4 so[kCombineWarps][R / 4];
+  if (lane == 0) {
+    sm[warp] = m;
+    sl[warp] = l;
   }
+#pragma unroll
+  for (int v = 0; v < V; ++v) so[warp][v * 32 + lane] = o[v];
+  __syncthreads();
+  if (warp >= V) return;  // warp v merges columns [128 v, 128 v + 128)
+  float top = -INFINITY, den = 0.0f;
+  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < kCombineWarps; ++i) top = fmaxf(top, sm[i]);
+  for (int i = 0; i < kCombineWarps; ++i) {
+    if (sm[i] == -INFINITY) continue;  // no partial
+    const float c = fast_exp2(sm[i] - top);
+    const float4 x = so[i][warp * 32 + lane];
+    den += sl[i] * c;
+    r.x += x.x * c;
+    r.y += x.y * c;
+    r.z += x.z * c;
+    r.w += x.w * c;
+  }
+  store_bf16x4(dst + warp * 128, r, 1.0f / den);
 }
 
 // The scratch: the sequences' runs, then every CTA's two partials.  One size for
@@ -1048,13 +1089,14 @@ int launch(dsb_ctx* ctx, const void* q_lat, const void* q_rope, const void* cach
                                static_cast<const __nv_bfloat16*>(q_rope), scales, n_blocks, block_table, max_blocks,
                                seq_lens, B, H, runs, softmax_scale * 1.4426950408889634f,
                                static_cast<__nv_bfloat16*>(out), ws_o, ws_ml, seq_runs, ctx->d_status));
-  auto combine = [&](auto kernel, unsigned y) {
-    return launch_pdl(kernel, dim3((unsigned)B, y), kCombineWarps * 32, 0, ctx->stream, seq_runs, H, HB, runs, ws_o,
-                      ws_ml, static_cast<__nv_bfloat16*>(out));
+  auto combine = [&](auto kernel, int heads, int threads) {  // heads per CTA
+    return launch_pdl(kernel, dim3((unsigned)B, (unsigned)((H + heads - 1) / heads)), threads, 0, ctx->stream, seq_runs,
+                      H, HB, runs, ws_o, ws_ml, static_cast<__nv_bfloat16*>(out));
   };
   // a sequence has about runs / B partials
-  if (B >= 32) DSB_CUDA_TRY(ctx, combine(combine_kernel<R, true>, (unsigned)((H + kCombineWarps - 1) / kCombineWarps)));
-  else DSB_CUDA_TRY(ctx, combine(combine_kernel<R, false>, (unsigned)H));
+  if (B < kFewFrom) DSB_CUDA_TRY(ctx, combine(combine_many_kernel<R>, 1, kCombineWarps * 32));
+  else if (B * H <= kSplitRows) DSB_CUDA_TRY(ctx, combine(combine_few_kernel<R, 1>, 512 / R, 128));
+  else DSB_CUDA_TRY(ctx, combine(combine_few_kernel<R, R / 128>, 8, 256));
   ctx->stats.kernel_launches += 2;
   ctx->stats.mla_calls++;
   return DSB_OK;
