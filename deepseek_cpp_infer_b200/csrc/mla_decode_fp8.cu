@@ -953,6 +953,7 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 256, V == 1 ? 10 : 4)
                        const float2* __restrict__ ws_ml, __nv_bfloat16* __restrict__ out) {
   pdl_wait();
   pdl_launch_dependents();
+  static_assert(V == 1 || V * 128 == R, "a warp of 8 takes whole heads");
   constexpr int kPerHead = R / 128 / V, kWarps = V == 1 ? 4 : 8;  // warps
   const int warp = (int)warp_id(), lane = (int)lane_id();
   const int b = blockIdx.x, h = blockIdx.y * (kWarps / kPerHead) + warp / kPerHead;
@@ -1094,9 +1095,15 @@ int launch(dsb_ctx* ctx, const void* q_lat, const void* q_rope, const void* cach
                       H, HB, runs, ws_o, ws_ml, static_cast<__nv_bfloat16*>(out));
   };
   // a sequence has about runs / B partials
-  if (B < kFewFrom) DSB_CUDA_TRY(ctx, combine(combine_many_kernel<R>, 1, kCombineWarps * 32));
-  else if (B * H <= kSplitRows) DSB_CUDA_TRY(ctx, combine(combine_few_kernel<R, 1>, 512 / R, 128));
-  else DSB_CUDA_TRY(ctx, combine(combine_few_kernel<R, R / 128>, 8, 256));
+  cudaError_t err = cudaSuccess;
+  if (B < kFewFrom) {
+    err = combine(combine_many_kernel<R>, 1, kCombineWarps * 32);
+  } else if (R == 128 || B * H <= kSplitRows) {
+    err = combine(combine_few_kernel<R, 1>, 512 / R, 128);
+  } else {
+    if constexpr (R == 512) err = combine(combine_few_kernel<R, 4>, 8, 256);
+  }
+  DSB_CUDA_TRY(ctx, err);
   ctx->stats.kernel_launches += 2;
   ctx->stats.mla_calls++;
   return DSB_OK;

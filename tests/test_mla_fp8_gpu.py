@@ -203,6 +203,20 @@ def test_decode_splits(gpu_ctx, lens, H):
     check_decode(out, *x[:5], lens, x[5])
 
 
+@pytest.mark.parametrize("shape", [BIG, SMALL])
+@pytest.mark.parametrize("B,H", [(31, 16), (32, 16), (40, 51), (40, 53), (64, 33), (33, 128), (700, 3)])
+def test_decode_merges(gpu_ctx, B, H, shape):
+    """Sequences cut by several runs, whole ones and empty ones, on both sides of the sizes at which the merge of the
+    cut ones changes its shape (32 sequences; 2048 rows)."""
+    lens = [(0, 1500, 40, 129, 333)[i % 5] + i % 3 for i in range(B)]
+    lens[0] = 0
+    x = decode_inputs(lens, H, shape, seed=B + H)
+    out = run_decode(gpu_ctx, *x[:5], lens, x[5])
+    gpu_ctx.sync()
+    check_decode(out, *x[:5], lens, x[5])
+    assert (out[0] == 0).all()
+
+
 def test_decode_ignores_what_lies_past_a_length(gpu_ctx):
     """Rows behind a length hold e4m3 NaN codes, infinite rope keys and NaN scales; table slots behind it are -1."""
     import torch
