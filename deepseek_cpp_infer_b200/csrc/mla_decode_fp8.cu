@@ -36,14 +36,14 @@
 // and, as soon as its block of O^T is done, is free again.
 //
 // What bounds it.  16 heads (12 slabs): HBM; 64 sequences of 1024 .. 8192
-// tokens take 41 us, 4.8 TB/s with all overheads, and a tile's 3100 cycles in
+// tokens take 40 us, 4.9 TB/s with all overheads, and a tile's 3100 cycles in
 // mid-run are the copy rate.  64 heads (72 KB of query digits leave 8 slabs):
 // the chain of a tile, about 5000 cycles against 2840 of MMAs: PV's first block
 // frees a slab, the next tile's last slab is loaded into it (1300 - 1900), QK,
 // softmax (1900), PV.  128 heads, the same sequences: 121 us, 697 TFLOP/s; 32 of
 // 4112 tokens 65 us; 3 of 60000 .. 131072 tokens 107 us.  At a sequence's end a
 // run takes another 14000 cycles for its output and the next query's digits.
-// One short sequence takes 11.5 us with the merge, two launches and a tile's
+// One short sequence takes 11.1 us with the merge, two launches and a tile's
 // chain.
 // What did not help: O^T accumulated in registers per tile, one warp for QK
 // and PV, four softmax warpgroups, 48 heads per CTA (9 slabs, 138 us), a
@@ -103,9 +103,13 @@ struct Shape {
   static constexpr int SMEM_BYTES = OFF_MISC + 128 + 1024;               // + alignment slack
   static_assert(SMEM_BYTES <= 232448, "shared memory");
   static_assert(OFF_Q8 % 1024 == 0 && OFF_QR % 1024 == 0 && OFF_P % 128 == 0 && OFF_SC % 16 == 0, "alignment");
-  // TMEM columns: S^T two buffers of [hi | lo], then O^T, one block of HB columns per latent slab
+  // TMEM columns: S^T two buffers of [hi | lo], then O^T per latent slab.  Where
+  // there is room both digits of the probabilities are columns of one MMA (42
+  // cycles up to N = 32, 50 at 64, 66 at 128) and O^T is [hi | lo] too: 16 heads
+  // x 777 tokens 11.4 -> 11.1 us, x 64 sequences 41.1 -> 40.3.
+  static constexpr int DIG = 4 * HB + 2 * NL * HB <= 512 ? 2 : 1;  // blocks of HB columns per slab
   static constexpr uint32_t T_S = 0, T_O = 4 * HB;
-  static constexpr int USED = 4 * HB + NL * HB;
+  static constexpr int USED = 4 * HB + NL * DIG * HB;
   static constexpr uint32_t T_COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
   static_assert(USED <= 512, "TMEM");
 };
@@ -475,9 +479,10 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
   } else if (warp == kPvWarp) {
     // --------------------------------------------------- PV: O^T of the segment
     if (count > 0 && elect_one()) {
-      constexpr uint32_t ID_PV = idesc_e4m3_f32(128, HB) | (1u << 15) | (1u << 16);  // A and B MN-major
+      constexpr int DIG = S::DIG;
+      constexpr uint32_t ID_PV = idesc_e4m3_f32(128, DIG * HB) | (1u << 15) | (1u << 16);  // A and B MN-major
       // P digits, no swizzle: 16 heads x 8 tokens per 128-byte core matrix,
-      // token groups 128 bytes apart, head groups 2048
+      // token groups 128 bytes apart, head groups 2048 (the lo digits' behind the hi ones')
       const uint64_t d_p = smem_desc(smem_base + S::OFF_P, 128, kTileTok * 16, kSwizzleNone);
       const uint64_t d_slab = smem_desc(smem_base + S::OFF_RING, 16, 1024, kSwizzle128B);
       auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait(bar, parity, abort); };
@@ -498,11 +503,12 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
 #pragma unroll
         for (int g = 0; g < NL; ++g) {
           const uint64_t a = d_slab + ((uint32_t)(slot[g] * S::SLAB) >> 4);
-          const uint32_t d = tmem + S::T_O + (uint32_t)(g * HB);
+          const uint32_t d = tmem + S::T_O + (uint32_t)(g * DIG * HB);
 #pragma unroll
           for (int ks = 0; ks < kTileTok / 32; ++ks) {
             mma_f8_ss(d, a + ks * (4096 >> 4), d_p + ks * (512 >> 4), ID_PV, first && ks == 0 ? 0u : 1u);
-            mma_f8_ss(d, a + ks * (4096 >> 4), d_p + (S::P_BYTES >> 4) + ks * (512 >> 4), ID_PV, 1u);
+            if constexpr (DIG == 1)
+              mma_f8_ss(d, a + ks * (4096 >> 4), d_p + (S::P_BYTES >> 4) + ks * (512 >> 4), ID_PV, 1u);
           }
           tc_commit(&empty[slot[g]]);
         }
@@ -755,20 +761,15 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
               fs[i] = __shfl_sync(0xffffffffu, f, c + i);
               ls[c + i] *= fs[i];
             }
-            constexpr int NB = 1;  // blocks read at once
 #pragma unroll 1
-            for (int g = 0; g < NL; g += NB) {
+            for (int g = 0; g < NL * S::DIG; ++g) {
               const uint32_t at = t_lane + S::T_O + g * HB + wg * HW + c;
-              uint32_t o[NB][8];
-#pragma unroll
-              for (int k = 0; k < NB; ++k) tmem_ld8(at + k * HB, o[k]);
+              uint32_t o[8];
+              tmem_ld8(at, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < NB; ++k) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[k][i] = __float_as_uint(__uint_as_float(o[k][i]) * fs[i]);
-                tmem_st8(at + k * HB, o[k]);
-              }
+              for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fs[i]);
+              tmem_st8(at, o);
             }
           }
           if (!first) tmem_st_wait();
@@ -870,8 +871,16 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
 #pragma unroll 1
       for (int g = 0; g < NL; ++g) {
         uint32_t o[HW];
-        tmem_ld(t_lane + S::T_O + g * HB + wg * HW, o);
-        tmem_ld_wait();
+        tmem_ld(t_lane + S::T_O + g * S::DIG * HB + wg * HW, o);
+        if constexpr (S::DIG == 2) {
+          uint32_t lo[HW];
+          tmem_ld(t_lane + S::T_O + g * S::DIG * HB + HB + wg * HW, lo);
+          tmem_ld_wait();
+#pragma unroll
+          for (int h = 0; h < HW; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) + __uint_as_float(lo[h]));
+        } else {
+          tmem_ld_wait();
+        }
         if (whole) {
           // four lanes swap so that each stores four latents of one head
           const bool s1 = lane & 1, s2 = lane & 2;
@@ -935,8 +944,8 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
 // 8th partial.
 // Bound by latency for small batches: with V = 1 a CTA (128 threads, 48
 // registers, no shared memory) is resident beside a decode CTA before that ends
-// (32 sequences x 16 heads 16.4 us with the decode kernel, 64 x 16 40.9; whole
-// heads 18.1, 42.6).  Bound by the partials' bytes out of L2 for large ones, where
+// (with the decode kernel then, 32 sequences x 16 heads 16.4 us, 64 x 16 40.9;
+// whole heads 18.1, 42.6).  Bound by the partials' bytes out of L2 for large ones, where
 // so many CTAs cost more (64 x 64 75.1 against 77.4 us, 74 x 128 whole sequences
 // 15.5 against 24.0).  Without the merge those four take 12.5, 37.7, 69.8, 13.4.
 constexpr int kCombineWarps = 8;
