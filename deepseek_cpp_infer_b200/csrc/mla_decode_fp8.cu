@@ -114,12 +114,6 @@ struct Shape {
   static_assert(USED <= 512, "TMEM");
 };
 
-__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -689,52 +683,20 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
             for (int h = 0; h < HW; ++h) u[h] = j < valid ? u[h] : -INFINITY;
           }
         }
-        // the tile's maximum per head (against r), over the warp's tokens and
-        // then the warpgroup's: two heads per register in fp16, whose error
-        // (2^-11 of the value) only matters far from r; lane head % HW gets it
-        uint32_t mx[HW / 2];
-#pragma unroll
-        for (int h = 0; h < HW / 2; ++h) mx[h] = pack_half2(u[2 * h], u[2 * h + 1]);
-#pragma unroll
-        for (int o = HW / 2; o >= 2; o >>= 1) {
-          const bool up = (lane & o) != 0;
-#pragma unroll
-          for (int h = 0; h < o / 2; ++h) {
-            const uint32_t give = up ? mx[h] : mx[h + o / 2], keep = up ? mx[h + o / 2] : mx[h];
-            mx[h] = max_half2(keep, __shfl_xor_sync(0xffffffffu, give, o));
-          }
-        }
-        mx[0] = max_half2(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], 1));
-#pragma unroll
-        for (int o = HW; o < 32; o <<= 1) mx[0] = max_half2(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
-        const float2 two = unpack_half2(mx[0]);
-        float mine = (lane & 1) ? two.y : two.x;
+        // the tile's maximum per head (against r): the warp's by reductions that
+        // do not wait for one another, then the warpgroup's (lane head % HW)
         const int hl = lane % HW;
         float* red_n = red + ((n & 1) * NWG + wg) * 4 * HW;
-        if (lane < HW) red_n[quarter * HW + lane] = mine;
+#pragma unroll
+        for (int h = 0; h < HW; h += 4) {
+          const float4 m = make_float4(redux_max(u[h]), redux_max(u[h + 1]), redux_max(u[h + 2]), redux_max(u[h + 3]));
+          if (lane == 0) *reinterpret_cast<float4*>(red_n + quarter * HW + h) = m;
+        }
         warp_arrive(&wg_bar[wg]);
         if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
         ++meet;
         float t = fmaxf(fmaxf(red_n[hl], red_n[HW + hl]), fmaxf(red_n[2 * HW + hl], red_n[3 * HW + hl]));
-        if (__any_sync(0xffffffffu, fabsf(t) > 1000.0f)) {
-          // far from the reference (a first tile with large scores, a jump, or
-          // past fp16's range): the maxima once more, in fp32
-#pragma unroll
-          for (int h = 0; h < HW; ++h) {
-            const float r = redux_max(u[h]);
-            if (hl == h) mine = r;
-          }
-          // the warpgroup's four warps are all here: they read the same maxima
-          warp_arrive(&wg_bar[wg]);
-          if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
-          ++meet;
-          if (lane < HW) red_n[quarter * HW + lane] = mine;
-          warp_arrive(&wg_bar[wg]);
-          if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
-          ++meet;
-          t = fmaxf(fmaxf(red_n[hl], red_n[HW + hl]), fmaxf(red_n[2 * HW + hl], red_n[3 * HW + hl]));
-          if (t == -INFINITY) t = 0.0f;
-        }
+        if (t == -INFINITY) t = 0.0f;
         r_top = first ? t + r_ref : fmaxf(r_top, t + r_ref);
         const float want = fmaxf(t, r_top - 40.0f - r_ref);
         const bool move = first || !(want >= kLow && want <= kHigh);
