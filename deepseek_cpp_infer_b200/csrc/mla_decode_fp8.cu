@@ -85,6 +85,7 @@ struct Shape {
   static constexpr int SLAB = kTileTok * 128;        // bytes
   static constexpr int NS = HB == 16 ? 12 : HB == 32 || NL == 1 ? 10 : 8;  // ring slots: what fits
   static_assert(NS >= NSLAB + 1, "ring");
+  static constexpr bool LATE = NS < 2 * NSLAB - 1;  // a tile's last slab waits for the last tile's PV
   static constexpr int Q8_BYTES = 2 * HB * R;        // [slab][hi heads | lo heads][128 B], SW128
   static constexpr int QR_BYTES = HB * P * 2;        // [head][P bf16], SW128 (P = 64) or SW64
   static constexpr int P_BYTES = HB * kTileTok;      // one digit of the probabilities
@@ -145,6 +146,12 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                    smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// Bring a box into L2 ahead of its load.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y)
                : "memory");
 }
 
@@ -395,15 +402,19 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
 #pragma unroll 1
         for (int k = 0; k < NSLAB; ++k, ++it) {
           const int slot = at_slab.slot;
+          const int row = k == 0 ? P * 2 : 128;  // bytes of a slab's row
+          const int x = k == 0 ? R : (k - 1) * 128;
+          const CUtensorMap* map = k == 0 ? &map_rope : &map_lat;
+          if (S::LATE && k == NSLAB - 1 &&  it >= NS && elect_one()) {
+            tma_prefetch_2d(map, x, page[0] * kPageTok);
+            if (np == 2) tma_prefetch_2d(map, x, page[1] * kPageTok);
+          }
           if (it >= NS && !__all_sync(0xffffffffu, mbar_wait(&empty[slot], at_slab.phase ^ 1u, abort))) {
             ok = false;
             break;
           }
           at_slab.step(1);
           uint8_t* dst = smem + S::OFF_RING + slot * S::SLAB;
-          const int row = k == 0 ? P * 2 : 128;  // bytes of a slab's row
-          const int x = k == 0 ? R : (k - 1) * 128;
-          const CUtensorMap* map = k == 0 ? &map_rope : &map_lat;
           if (elect_one()) {
             mbar_arrive_expect_tx(&full[slot], np * kPageTok * row);
             tma_load_2d(dst, map, &full[slot], x, page[0] * kPageTok, policy);
