@@ -7,7 +7,7 @@
 // The cached bytes are tensor-core operands as they are stored; nothing is
 // converted.  Tokens are the MMA's M: a tile is 128 tokens (two pages), and
 //   S^T [128 tokens x heads] = C8 . Q^T  (+ KR . Qr^T, kind::f16)
-//   O^T [R x heads] per tile  = C8^T . P (the same bytes, MN-major)
+//   O^T [R x heads] += C8^T . P          (the same bytes, MN-major)
 // so that few heads cost few columns and the tile is read once for both
 // products.
 //
@@ -27,7 +27,7 @@
 // group of up to 64 heads; both groups of 128 heads walk the same tiles at
 // the same time and share them through L2).  The lengths are read on the
 // device.  A run's first and last sequences may be shared with its neighbours:
-// such segments go to fp32 partials that combine_kernel merges.
+// such segments go to fp32 partials that a second kernel merges.
 //
 // Roles (11 warps): 8 softmax warps, two warpgroups with half the heads each
 // (thread = token for S^T, thread = latent column for O^T), a TMA warp, a warp
@@ -36,12 +36,12 @@
 // and, as soon as its block of O^T is done, is free again.
 //
 // What bounds it.  16 heads (12 slabs): HBM; 64 sequences of 1024 .. 8192
-// tokens take 40 us, 4.9 TB/s with all overheads, and a tile's 3100 cycles in
+// tokens take 39 us, 5.0 TB/s with all overheads, and a tile's 3100 cycles in
 // mid-run are the copy rate.  64 heads (72 KB of query digits leave 8 slabs):
 // the chain of a tile, about 5000 cycles against 2840 of MMAs: PV's first block
 // frees a slab, the next tile's last slab is loaded into it (1300 - 1900), QK,
-// softmax (1900), PV.  128 heads, the same sequences: 121 us, 697 TFLOP/s; 32 of
-// 4112 tokens 65 us; 3 of 60000 .. 131072 tokens 107 us.  At a sequence's end a
+// softmax (1900), PV.  128 heads, the same sequences: 120 us, 700 TFLOP/s; 32 of
+// 4112 tokens 64 us; 3 of 60000 .. 131072 tokens 107 us.  At a sequence's end a
 // run takes another 14000 cycles for its output and the next query's digits.
 // One short sequence takes 11.1 us with the merge, two launches and a tile's
 // chain.
@@ -51,7 +51,9 @@
 // float4 (134 us).  At 64 heads the softmax warps use all 168 registers that
 // three warps a partition leave: more loads in flight for the query's digits
 // spill, and any spill beside 228 KB of shared memory costs 5% or more
-// (setmaxnreg with a twelfth warp: 139 us); tiles prefetched into L2 (127 us).
+// (setmaxnreg with a twelfth warp: 139 us; the query's digits between the
+// output's blocks: 123 us).  Whole tiles prefetched into L2 cost more of its
+// bandwidth than they save (127 us).
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -227,7 +229,7 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 
 // First tile of run i of n over T tiles.
 __device__ __forceinline__ int64_t run_start(int64_t i, int64_t T, int n) { return i * T / n; }
-// What combine_kernel has to do for a sequence: its first partial's slot and
+// What the merge has to do for a sequence: its first partial's slot and
 // its last run (written by the runs that begin and end it), or one of these.
 constexpr int kSeqEmpty = -1, kSeqWhole = -2;
 
