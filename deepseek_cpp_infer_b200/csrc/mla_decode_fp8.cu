@@ -111,6 +111,9 @@ struct Shape {
   // cycles up to N = 32, 50 at 64, 66 at 128) and O^T is [hi | lo] too: 16 heads
   // x 777 tokens 11.4 -> 11.1 us, x 64 sequences 41.1 -> 40.3.
   static constexpr int DIG = 4 * HB + 2 * NL * HB <= 512 ? 2 : 1;  // blocks of HB columns per slab
+  // In columns of their own the lo digits are held 16-fold (a remainder is at
+  // most 16: half a step of 256 .. 448), which moves their floor down as much.
+  static constexpr int LO = DIG == 2 ? 16 : 1;
   static constexpr uint32_t T_S = 0, T_O = 4 * HB;
   static constexpr int USED = 4 * HB + NL * DIG * HB;
   static constexpr uint32_t T_COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
@@ -129,8 +132,9 @@ __device__ __forceinline__ float redux_max(float v) {
   return r;
 }
 
-// Two floats as e4m3 digits: hi = e4m3(v), lo = e4m3(v - hi), through fp16 (11
-// significant bits; the difference is exact).
+// Two floats as e4m3 digits: hi = e4m3(v), lo = e4m3((v - hi) * LO), through
+// fp16 (11 significant bits; the difference is exact).
+template <int LO = 1>
 __device__ __forceinline__ void split_digits(float a, float b, uint32_t& hi, uint32_t& lo) {
   const uint32_t v = pack_half2(a, b);
   uint16_t h, l;
@@ -138,6 +142,7 @@ __device__ __forceinline__ void split_digits(float a, float b, uint32_t& hi, uin
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(v));
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hf) : "h"(h));
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(hf));
+  if constexpr (LO == 16) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(d), "r"(0x4c004c00u));
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(l) : "r"(d));
   hi = h;
   lo = l;
@@ -629,12 +634,14 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
 
     // Probabilities and sums are in units of 2^r, r a per-head reference (held
     // by lane head % HW) that keeps each tile's largest probability between
-    // 1 and 430: its digits then hold it to 2^-10, and what is smaller than
-    // 2^-4 of the largest to a 2^-14th of it, whatever came before.  When a
-    // tile's maximum leaves that window, the reference moves (to make it 16)
-    // and the head's columns of O^T are rescaled in TMEM; fp32 has the range
-    // for both directions (r never falls more than 2^40 below the largest:
-    // what lies further down is out of an fp32 sum's reach).
+    // 1 and 430, whatever came before: a probability's digits are then off by
+    // at most 2^-8 of it, or 2^-10 (2^-14 with lo held 16-fold) where that is
+    // more.  (So with lo held plainly, equal probabilities of 2^-6 beside one of 1
+    // in every tile can all be off by 2^-4 of themselves; roundings that differ
+    // average out.)  When a tile's maximum leaves that window, the reference
+    // moves (to make it 16) and the head's columns of O^T are rescaled in TMEM;
+    // fp32 has the range for both directions (r never falls more than 2^40 below
+    // the largest: what lies further down is out of an fp32 sum's reach).
     constexpr float kNew = 4.0f, kHigh = 8.75f, kLow = 0.0f;  // of the tile's maximum, in log2
     float ls[HW];  // softmax sums over this thread's tokens
     float r_ref = 0.0f, r_top = 0.0f;
@@ -761,8 +768,8 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           u[h + 2] = fast_exp2(u[h + 2]);
           u[h + 3] = fast_exp2(u[h + 3]);
           uint32_t a, b2, c, d;
-          split_digits(u[h + 0], u[h + 1], a, b2);
-          split_digits(u[h + 2], u[h + 3], c, d);
+          split_digits<S::LO>(u[h + 0], u[h + 1], a, b2);
+          split_digits<S::LO>(u[h + 2], u[h + 3], c, d);
           hi[h / 4] = a | (c << 16);
           lo[h / 4] = b2 | (d << 16);
         }
@@ -852,7 +859,8 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           tmem_ld(t_lane + S::T_O + g * S::DIG * HB + HB + wg * HW, lo);
           tmem_ld_wait();
 #pragma unroll
-          for (int h = 0; h < HW; ++h) o[h] = __float_as_uint(__uint_as_float(o[h]) + __uint_as_float(lo[h]));
+          for (int h = 0; h < HW; ++h)
+            o[h] = __float_as_uint(__uint_as_float(o[h]) + __uint_as_float(lo[h]) * (1.0f / S::LO));
         } else {
           tmem_ld_wait();
         }

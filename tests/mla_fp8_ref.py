@@ -85,9 +85,9 @@ def decode64(q_lat, q_rope, cache, scales, table, lens, scale):
 def decode_tol(out, mag, top):
     """Elementwise bound of |kernel - out|.  The output's bf16 rounding: 2^-8 |out|.  A probability is held as the
     sum of two e4m3 digits, the second rounding the first's remainder (2^-4 of it, itself at most 2^-4 of the
-    probability): 2^-8 of each term, so 2^-8 mag.  Below the digits' range (e4m3's smallest step, 2^-9) each is off
-    by at most 2^-10 in units in which its tile's largest is between 1 and 430, upwards or downwards; the terms of
-    a sequence must cancel to 2^-11 top, which is stricter than their worst case.  Scores carry fp32 sums of exact products (the two digits of
+    probability): 2^-8 of each term, so 2^-8 mag.  Below the digits' range each is off by at most 2^-14 of its tile's
+    largest (2^-10 at 64 heads a CTA), upwards or downwards; the terms of a sequence must cancel to 2^-11 top, which is
+    stricter than their worst case.  Scores carry fp32 sums of exact products (the two digits of
     a query are exact to 2^-18 of its largest value): 2^-12 mag covers sum |q k| scale up to about 500."""
     return 2.0 ** -8 * out.abs() + (2.0 ** -8 + 2.0 ** -12) * mag + 2.0 ** -11 * top[:, None, None] + 1e-30
 

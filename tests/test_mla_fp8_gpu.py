@@ -256,6 +256,42 @@ def test_decode_attention_sink(gpu_ctx):
     check_decode(out, q_lat, q_rope, cache, scales, table, [n], scale)
 
 
+@pytest.mark.parametrize("H", [16, 64])
+def test_decode_equal_tail_beside_a_peak_in_every_tile(gpu_ctx, H):
+    """Equal probabilities whose digits all round the same way, in tiles whose largest is at the low end of the digits'
+    window.  Up to 32 heads their floor is 2^-14 of the window's unit and the common bound holds; at 64 each may be
+    off by 2^-10 of a unit that is at most its tile's largest: 2^-10 sum_j top(tile of j) |latent_j| more."""
+    import torch
+
+    B, n, R = torch.cuda.get_device_properties(0).multi_processor_count, 1024, 512  # a sequence of 8 tiles for every SM
+    lens = [n] * B
+    q_lat, q_rope, cache, scales, table, scale = decode_inputs(lens, H, BIG, seed=8)
+    q_lat.zero_()
+    q_rope.zero_()
+    q_rope[..., 0] = 1.0
+    # the first tile's largest probability is 16 units, the others' 1.05, the tail 8.5 steps of 2^-9
+    unit = torch.full((n,), 8.5 * 2.0 ** -9, dtype=torch.float64)
+    unit[5::128] = 1.05
+    unit[5] = 16.0
+    kr = torch.zeros(cache.shape[0], 64, 64, device="cuda")
+    kr[table.long(), :, 0] = (unit.log() / scale).float().cuda().view(1, -1, 64).expand(B, -1, -1)
+    codes, sc = ref.quantise(torch.randn(cache.shape[0], 64, R, device="cuda", dtype=torch.float64) * 0.1 + 1.0)
+    sc.fill_(2.0 ** -8)  # (any power of two: the codes stand for other values then)
+    cache[..., :R], scales[:] = codes, sc
+    cache[..., R:] = (kr / sc[..., None]).bfloat16().view(torch.uint8)
+    out = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, lens, scale)
+    gpu_ctx.sync()
+    want, mag, top = ref.decode64(q_lat, q_rope, cache, scales, table, lens, scale)
+    tol = ref.decode_tol(want, mag, top)
+    if H == 64:
+        for b in range(B):
+            lat, rope = ref.rows64(cache, scales, table, b, n, R)
+            p = torch.softmax(rope[:, 0] * scale, -1).view(-1, 128)
+            tol[b] += 2.0 ** -10 * (p.amax(1, keepdim=True).expand(-1, 128).reshape(-1) @ lat.abs())
+    err = (out.double() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
 def test_decode_scales_far_apart(gpu_ctx):
     """Token scales over 20 octaves and queries over 8: the largest tokens' latents dominate the output."""
     import torch
