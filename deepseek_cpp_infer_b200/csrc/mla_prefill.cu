@@ -24,9 +24,9 @@
 // prologue overlaps the last one's epilogue.
 //
 // Bound by the tensor core and, before it, by power: at 128 heads one prompt
-// of 4096 rows (causal) takes 730 us and 1024 rows behind 3000 keys 300 us,
-// 940 - 1000 TFLOP/s at 1.6 - 1.75 GHz under the 1000 W limit (cuBLAS sustains
-// 1386 there); 32 prompts of about 512 rows at 16 heads 96 us, 2.3 times the
+// of 4096 rows (causal) takes 708 us and 1024 rows behind 3000 keys 283 us,
+// 970 - 1050 TFLOP/s at 1.6 - 1.75 GHz under the 1000 W limit (cuBLAS sustains
+// 1386 there); 32 prompts of 512 rows at 16 heads 85 us, 1.8 times the
 // time of their bytes: an item is only 1 to 4 steps long, so that its Q load,
 // first softmax and output show.  What did not help: an MMA warp for each tile
 // (15% slower: the tiles fall into step), two softmax warpgroups a tile, P
@@ -249,8 +249,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   bool ok = true;
   // 384 threads were launched with 168 registers each; the softmax warps hold
-  // a row's 128 scores: 256 * 208 + 128 * 88 = 384 * 168
-#define DSB_FEW_REGS asm volatile("setmaxnreg.dec.sync.aligned.u32 88;")
+  // a row's 128 scores: 256 * 192 + 128 * 120 = 384 * 168 (208 + 88 spill in the
+  // other roles: 32 prompts of 512 rows, 16 heads, 90.6 us instead of 85.4)
+#define DSB_FEW_REGS asm volatile("setmaxnreg.dec.sync.aligned.u32 120;")
 
   if (warp == kTmaWarp) {
     // ------------------------------------------------------------ TMA producer
@@ -279,6 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) {
         const int tiles = (x.n[0] > 0 ? 1 : 0) + (x.n[1] > 0 ? 1 : 0);
         mbar_arrive_expect_tx(q_full, tiles * S::K_BYTES);
+#pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (x.n[t] == 0) continue;
           uint8_t* dst = smem + S::OFF_Q + t * NQ * S::SLAB;
@@ -354,20 +356,36 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < NQ; ++i) tc_commit(&empty[k_slot[i]]);
       };
-      for (int it = blockIdx.x; ok && it < items; it += gridDim.x) {
-        Item x;
-        bool bad;
-        if (!get_item(a, order, it, &x, &bad) || x.steps() == 0) continue;
-        const int n = x.steps();
+      int it = blockIdx.x;
+      // Of an item this role needs its tiles' steps and the keys that all rows see.
+      // Finding them takes 1400 cycles (the lengths, five divisions): it is done
+      // for the next item while this one's first softmax runs.
+      int n_next[2], keys_next;
+      auto find_next = [&] {
+        for (; it < items; it += gridDim.x) {
+          Item x;
+          bool bad;
+          if (!get_item(a, order, it, &x, &bad) || x.steps() == 0) continue;
+          n_next[0] = x.n[0];
+          n_next[1] = x.n[1];
+          keys_next = x.common(causal);
+          return true;
+        }
+        return false;
+      };
+      bool have = find_next();
+      while (ok && have) {
+        const int n_of[2] = {n_next[0], n_next[1]}, n = max(n_of[0], n_of[1]), full_keys = keys_next;
         ok = wait(q_full, n_item & 1u) && wait_k();
         if (!ok) break;
         ++n_item;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-          if (x.n[t] > 0) issue_qk(t);
+          if (n_of[t] > 0) issue_qk(t);
         release_k();
         if (n == 1) tc_commit(q_empty);
-        const int full_keys = x.common(causal);
+        it += gridDim.x;
+        have = find_next();
         for (int s = 0; ok && s < n; ++s) {
           // V of this step
           v_slot = ring.take(NV);
@@ -384,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool more = s + 1 < n;
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            if (ok && s < x.n[t]) {
+            if (ok && s < n_of[t]) {
               if (s == 0 && item_of[t]++ > 0) ok = wait(&o_free[t], (item_of[t] - 2) & 1u);
               ok = ok && wait(&p_full[t], step_of[t] & 1u);
               if (!ok) break;
@@ -404,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (ok && more) {
               // the next scores of this tile, while the other tile's softmax runs
               if (t == 0) ok = wait_k();
-              if (ok && s + 1 < x.n[t]) issue_qk(t);
+              if (ok && s + 1 < n_of[t]) issue_qk(t);
               if (ok && t == 1) {
                 release_k();
                 if (s + 2 == n) tc_commit(q_empty);
@@ -505,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) raise_abort(abort, status, kStatusTimeout);
   } else {
     // ---------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int t = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;  // row of the tile == TMEM lane
     const uint32_t tl = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -518,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int i = x.row0 + t * kRows + r;  // row within the sequence
       const bool live = i < x.rows;
       const int64_t row = (int64_t)x.q0 + i;
-      const int n = x.n[t];
+      const int n = t == 0 ? x.n[0] : x.n[1];
       const int sees = x.sees(i, causal);
       float m = -INFINITY, l = 0.0f;  // m in the exp2 domain
       for (int s = 0; s < n; ++s, ++c) {
