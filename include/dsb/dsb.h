@@ -383,11 +383,12 @@ DSB_API int dsb_kv_norm_rope_append_fp8(dsb_ctx* ctx, const float* kv_a, int64_t
  * over the seq_lens[b] cached tokens of sequence b (a length of 0 gives a zero
  * row).  seq_lens is a DEVICE int32 [B]: the kernel splits the work itself, so
  * a captured call may be replayed with other lengths.  Cache rows past a
- * length are not used, whatever they hold.  A probability is held to 2^-8 of
- * its value, or 2^-14 (with R = 512 and more than 32 heads 2^-10) of the largest
- * among its 128 tokens where that is more; sums in fp32.  Scales must be positive; a token
- * whose scale is 2^-40 of its sequence's largest or less may count as a zero
- * row, one of scale 0 (a row never written) counts as 2^-100.  Scratch comes
+ * length are not used, whatever they hold.  A probability times its token's
+ * scale is held to 2^-8 of its value, or 2^-14 (with R = 512 and more than 32
+ * heads 2^-10) of the largest among its 128 tokens where that is more; sums are
+ * in fp32.  Scales must be positive; a token whose scale is 2^-40 of its
+ * sequence's largest or less may count as a zero row, one of scale 0 (a row
+ * never written) counts as 2^-100.  Scratch comes
  * from the context (39 MB, allocated by the first call): calls of one context
  * must not overlap on the GPU.  H <= 128, B <= 65536, B * max_blocks < 2^31,
  * lengths <= 2^30, n_blocks < 2^25; q_lat, q_rope, out_lat bf16 as in
