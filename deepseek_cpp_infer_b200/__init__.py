@@ -451,6 +451,8 @@ class Context:
               ("block_table", block_table, "int32", (rows, max_blocks), 0), ("kv_a", kv_a, "float32", (B, width), 1),
               ("w_norm", w_norm, "float32", (R,), 0), ("q", q, "bfloat16", (B, q.shape[-1]), 1),
               ("positions", positions, "int32", (B,), 0), ("q_rope", q_rope, "bfloat16", (B, H, P), 0))
+        if width < R + P or q.shape[1] < H * (nope + P):  # (a view's pitch does not show it)
+            raise ValueError(f"rows of {R + P} values (kv_a) and {H * (nope + P)} (q) wanted, got {width} and {q.shape[1]}")
         if seq_ids is not None:
             _need(self.device, ("seq_ids", seq_ids, "int32", (B,), 0))
         self._check(self._l.dsb_kv_norm_rope_append_fp8(

@@ -6,6 +6,7 @@ import os
 import subprocess
 
 import numpy as np
+import pytest
 
 import deepseek_cpp_infer_b200 as dsb
 import mla_fp8_ref as ref
@@ -77,3 +78,48 @@ def test_every_cached_value_is_exact_in_bf16():
     for e in (-64, -17, -1, 0, 9, 64):
         v = table * 2.0 ** e
         assert torch.equal(v.bfloat16().float(), v)
+
+
+class _Recorder:
+    """Stands in for the library: every entry point notes its arguments and succeeds."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return dsb.DSB_OK
+
+        return call
+
+
+def binding():
+    """A Context whose calls end before the library; its tensors lie on the host (device -1)."""
+    ctx = object.__new__(dsb.Context)
+    ctx._l, ctx.h, ctx.device = _Recorder(), None, -1
+    return ctx
+
+
+def append_args(H=2, B=3, R=128, P=32, nope=64):
+    import torch
+
+    return dict(kv_a=torch.zeros(B, R + P), w_norm=torch.ones(R), q=torch.zeros(B, H * (nope + P)).bfloat16(),
+                positions=torch.zeros(B, dtype=torch.int32), block_table=torch.zeros(B, 1, dtype=torch.int32), H=H,
+                nope=nope, R=R, P=P, eps=1e-6, theta=1e4, cache=torch.zeros(4, 64, R + 2 * P, dtype=torch.uint8),
+                scales=torch.ones(4, 64), q_rope=torch.zeros(B, H, P).bfloat16())
+
+
+@pytest.mark.parametrize("name,cut", [("kv_a", slice(64, None)), ("kv_a", slice(0, 156)), ("q", slice(96, None)),
+                                      ("q", slice(0, 184))])
+@pytest.mark.parametrize("B", [1, 3])
+def test_append_refuses_rows_narrower_than_a_token(name, cut, B):
+    """A view of part of each row has the whole row's pitch: only its width shows that the kernel would read the next
+    row's values, and behind the last row what follows the allocation."""
+    a = append_args(B=B)
+    ctx = binding()
+    ctx.kv_norm_rope_append_fp8(**a)
+    assert len(ctx._l.calls) == 1
+    with pytest.raises(ValueError, match=name):
+        ctx.kv_norm_rope_append_fp8(**{**a, name: a[name][:, cut]})
+    assert len(ctx._l.calls) == 1
