@@ -49,9 +49,12 @@ namespace {
 constexpr int kRows = 128;       // query rows per tile, keys per step
 constexpr int kThreads = 12 * 32;
 constexpr int kTmaWarp = 8, kMmaWarp = 9, kScanWarp = 10;
-// Non-finite values that were taken out of a bordering tile, per column: the
-// first key that has one (shifted by 3) and what kinds there are.
-constexpr uint32_t kPlusInf = 1, kMinusInf = 2, kNan = 4, kNothing = 0xffffffffu;
+// Non-finite values that were taken out of an item's bordering tiles, a word per
+// column: for +inf, -inf and NaN the first key that holds one, 10 bits each,
+// counted from the first bordering step.  (The border crosses at most 255 keys
+// behind the first step's common ones: three steps, 384 keys; 1023: none.)
+constexpr int kPlusInf = 0, kMinusInf = 10, kNan = 20;  // shifts
+constexpr uint32_t kKeyMask = 1023, kNothing = 0x3fffffffu;
 constexpr float kLazy = 8.0f;    // log2 headroom before O is rescaled
 
 template <int NOPE, int P, int VD>
@@ -102,6 +105,8 @@ struct Item {
   __device__ int steps() const { return max(n[0], n[1]); }
   // keys that all rows of the item see: a step that reaches further is a bordering one
   __device__ int common(bool causal) const { return min(lk, causal ? row0 + 1 + lk - lq : lk); }
+  // the first bordering step
+  __device__ int border(bool causal) const { return max(0, common(causal)) / kRows; }
   // keys that query row i of the sequence sees
   __device__ int sees(int i, bool causal) const { return causal ? max(0, min(lk, i + 1 + lk - lq)) : lk; }
 };
@@ -447,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool bad;
       if (!get_item(a, order, it, &x, &bad) || x.steps() == 0) continue;
       const int n = x.steps();
-      const int full_keys = x.common(causal);
+      const int full_keys = x.common(causal), border = x.border(causal);
       uint32_t* word = reinterpret_cast<uint32_t*>(smem + S::OFF_BAD + (n_item % 3) * S::BAD_BYTES);
       uint32_t* any = word + VD;
       const uint32_t turn = n_item % 3, use = n_item / 3;
@@ -498,13 +503,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t value = (w[i / 2] >> (16 * (i & 1))) & 0xffffu;
                 if ((value & 0x7f80u) != 0x7f80u) continue;
                 const int col = chunk * 8 + i;
-                const uint32_t kind = (value & 0x7fu) != 0 ? kNan : (value & 0x8000u) != 0 ? kMinusInf : kPlusInf;
-                const uint32_t key = (uint32_t)(s * kRows + row) << 3;
+                const int kind = (value & 0x7fu) != 0 ? kNan : (value & 0x8000u) != 0 ? kMinusInf : kPlusInf;
+                const uint32_t key = (uint32_t)((s - border) * kRows + row);
                 uint32_t old = word[col], now;
                 do {
                   now = old;
-                  const uint32_t merged = old == kNothing ? key | kind : min(old & ~7u, key) | (old & 7u) | kind;
-                  old = atomicCAS(&word[col], now, merged);
+                  const uint32_t first = min((now >> kind) & kKeyMask, key);
+                  old = atomicCAS(&word[col], now, (now & ~(kKeyMask << kind)) | (first << kind));
                 } while (old != now);
                 w[i / 2] &= (i & 1) ? 0x0000ffffu : 0xffff0000u;
               }
@@ -649,13 +654,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld32(to + 32 * k, o);
         tmem_ld_wait();
         if (fix) {
+          const int seen = sees - x.border(causal) * kRows;  // of the recorded keys
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const uint32_t b = word[32 * k + e];
-            if (b != kNothing && (int)(b >> 3) < sees) {
-              const float add = (b & kNan) != 0 || (b & (kPlusInf | kMinusInf)) == (kPlusInf | kMinusInf) ? NAN
-                                : (b & kPlusInf) != 0 ? INFINITY : -INFINITY;
-              o[e] = __float_as_uint(__uint_as_float(o[e]) + add);
+            if (b != kNothing) {
+              auto has = [&](int kind) { return (int)((b >> kind) & kKeyMask) < seen; };
+              float add = has(kPlusInf) ? INFINITY : 0.0f;
+              add += has(kMinusInf) ? -INFINITY : 0.0f;
+              o[e] = __float_as_uint(__uint_as_float(o[e]) + (has(kNan) ? NAN : add));
             }
           }
         }

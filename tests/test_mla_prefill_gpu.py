@@ -174,6 +174,44 @@ def test_masked_future_infinities_do_not_leak(gpu_ctx):
     assert torch.equal(out[:at], clean[:at]) and torch.equal(lse[:at], lc[:at])
 
 
+@pytest.mark.parametrize("lq,lk,keys,causal", [
+    (300, 300, [10, 50, 120], True),      # one bordering step
+    (300, 300, [100, 128, 255], True),    # over the steps that one item's border crosses
+    (200, 500, [310, 390, 480], True),    # behind a history
+    (256, 511, [254, 400, 510], True),    # the widest border: keys 256 .. 510, and one that every row sees
+    (130, 300, [0, 260, 299], True), (40, 333, [257, 300, 332], False)])
+def test_non_finite_values_reach_the_rows_that_see_them_only(gpu_ctx, lq, lk, keys, causal):
+    """Each column holds up to three of +inf, -inf and NaN at different keys, in every order.  A row's column is what
+    the values that the row sees make of it: NaN from a NaN or from both infinities, the infinity from one, the
+    clean result from none."""
+    import itertools
+
+    import torch
+
+    inf, nan = float("inf"), float("nan")
+    x = inputs([lq], [lk], 2, BIG, seed=lq + lk)
+    clean, lc = run(gpu_ctx, x, [lq], [lk], causal=causal)
+    order = list(itertools.permutations([inf, -inf, nan, None], 3))
+    want, row = clean.clone(), torch.arange(lq, device="cuda")
+    for col, kinds in enumerate(order):
+        total = torch.zeros(lq, device="cuda")
+        for key, value in zip(keys, kinds):
+            if value is not None:
+                x[4][key, :, col] = value
+                total += torch.where((row + lk - lq >= key) | (not causal), value, 0.0)
+        want[:lq, :, col] = torch.where((total == 0)[:, None], want[:lq, :, col], total[:, None].bfloat16())
+    out, lse = run(gpu_ctx, x, [lq], [lk], causal=causal)
+    gpu_ctx.sync()
+    assert torch.equal(lse, lc)
+    cut = len(order)
+    assert torch.equal(out[:, :, cut:], clean[:, :, cut:])
+    got, want = out[:lq, :, :cut].float(), want[:lq, :, :cut].float()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    assert torch.equal(got[~want.isnan()].sign(), want[~want.isnan()].sign())
+    # (a value that a row does not see has no weight there, whatever it was)
+    assert torch.equal(got[want.isfinite()], want[want.isfinite()])
+
+
 def test_long_prompt_and_repeats_are_bitwise(gpu_ctx):
     import torch
 
