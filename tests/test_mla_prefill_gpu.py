@@ -334,6 +334,71 @@ def test_refusals(gpu_ctx):
     gpu_ctx.sync()
 
 
+# ------------------------------------------- more items than SMs (each CTA takes several)
+
+
+def crowd(name):
+    """(lq, lk, H, dims): calls with several work items (256 query rows of a head) for every SM."""
+    import torch
+
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    rng = np.random.default_rng(len(name))
+    if name == "ragged":  # about eight items a CTA, dead ones (short and empty prompts) between live ones
+        lq = [0, 1, *rng.integers(100, 513, size=28).tolist(), 0, 257]
+        return lq, lq, (4 * sms + len(lq) - 1) // len(lq), BIG
+    if name == "groups":  # head groups of two items an SM, the last one short
+        return [600], [600], 128, BIG
+    if name == "sees_nothing":  # more queries than keys: tiles and whole items without keys beside ones with
+        lq, lk = [600, 300, 256, 40, 700, 129], [100, 301, 90, 0, 40, 513]
+        return lq, lk, (3 * sms + 17) // 18 + 1, BIG
+    if name == "history":
+        lq = rng.integers(1, 300, size=12).tolist()
+        return lq, [n + int(p) for n, p in zip(lq, rng.integers(0, 900, size=12))], (3 * sms + 11) // 12, BIG
+    lq = [0, 1, *rng.integers(100, 700, size=20).tolist(), 3]
+    return lq, lq, (4 * sms + len(lq) - 1) // len(lq), SMALL
+
+
+CROWDS = ["ragged", "groups", "sees_nothing", "history", "small"]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("name", CROWDS)
+def test_several_items_per_cta(gpu_ctx, name, causal):
+    import torch
+
+    lq, lk, H, dims = crowd(name)
+    x = inputs(lq, lk, H, dims, seed=100, extra=5)
+    out, lse = run(gpu_ctx, x, lq, lk, causal=causal)
+    gpu_ctx.sync()
+    check(out, lse, x, lq, lk, causal=causal)
+    again, l2 = run(gpu_ctx, x, lq, lk, causal=causal)
+    assert torch.equal(out, again) and torch.equal(lse, l2)
+
+
+@pytest.mark.parametrize("name", ["ragged", "history", "small"])
+def test_several_items_per_cta_with_non_finite_values(gpu_ctx, name):
+    """A NaN in some sequences' border and none in others, so that items with and without one follow each other on a
+    CTA: only its column, and only in rows that see it."""
+    import torch
+
+    lq, lk, H, dims = crowd(name)
+    x = inputs(lq, lk, H, dims, seed=101)
+    clean, lc = run(gpu_ctx, x, lq, lk)
+    want, q0, k0 = clean.clone(), 0, 0
+    for b, (n, m) in enumerate(zip(lq, lk)):
+        key = m - 1 - (7 * b) % max(1, n)  # the last n keys are bordering ones
+        if b % 3 != 0 and n > 0:
+            for h in range(b % 2, H, 2):
+                col = (5 * b + h) % x[4].shape[2]
+                x[4][k0 + key, h, col] = float("nan")
+                want[q0 + max(0, key - (m - n)):q0 + n, h, col] = float("nan")
+        q0, k0 = q0 + n, k0 + m
+    out, lse = run(gpu_ctx, x, lq, lk)
+    gpu_ctx.sync()
+    assert torch.equal(lse, lc) and torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out[~want.isnan()], want[~want.isnan()])
+
+
 # ------------------------------------------------------------- as a model runs them
 
 
