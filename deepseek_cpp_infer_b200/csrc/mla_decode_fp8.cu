@@ -1035,8 +1035,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
   float top = -INFINITY, den = 0.0f;
   float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = 0; i < kCombineWarps; ++i) top = fmaxf(top, sm[i]);
-  for (int i = 0; i < kCombineWarps; ++i) {
-    if (sm[i] == -INFINITY) continue;  // no partial
+  const int filled = min(kCombineWarps, i1 - i0 + 1);  // warps that had a partial (a NaN one's sm is -inf as well)
+  for (int i = 0; i < filled; ++i) {
     const float c = fast_exp2(sm[i] - top);
     const float4 x = so[i][warp * 32 + lane];
     den += sl[i] * c;

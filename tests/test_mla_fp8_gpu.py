@@ -437,6 +437,24 @@ def test_decode_non_finite_query_stays_in_its_head(gpu_ctx, value):
     check_decode(out, q_lat, q_rope, cache, scales, table, lens, scale)
 
 
+@pytest.mark.parametrize("B", [1, 31, 32, 40])
+@pytest.mark.parametrize("tiles", [[0], [3], [0, 5], [7]])
+def test_decode_nan_tile_of_a_cut_sequence(gpu_ctx, B, tiles):
+    """A tile of 128 tokens with NaN rope keys, each tile of its sequence in a run of its own: the sequence's output is
+    NaN whichever merge joins the runs, the other sequences' as without it."""
+    import torch
+
+    lens = [1000] + [1] * (B - 1)
+    q_lat, q_rope, cache, scales, table, scale = decode_inputs(lens, 16, BIG, seed=50 + B)
+    clean = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, lens, scale)
+    for t in tiles:
+        cache[table[0, 2 * t:2 * t + 2].long(), :, 512:] = 0xFF  # bf16 NaN
+    out = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, lens, scale)
+    gpu_ctx.sync()
+    assert out[0].isnan().all()
+    assert torch.equal(out[1:], clean[1:]) and clean.isfinite().all()
+
+
 def test_decode_length_beyond_32_bit_positions_is_reported(gpu_ctx):
     """A table of 2^24 + 1 pages would hold it; positions past 2^30 are refused instead of wrapping."""
     import torch
