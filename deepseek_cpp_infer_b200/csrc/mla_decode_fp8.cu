@@ -718,14 +718,18 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         float t = fmaxf(fmaxf(red_n[hl], red_n[HW + hl]), fmaxf(red_n[2 * HW + hl], red_n[3 * HW + hl]));
         if (t == -INFINITY) t = 0.0f;
         r_top = first ? t + r_ref : fmaxf(r_top, t + r_ref);
-        const float want = fmaxf(t, r_top - 40.0f - r_ref);
+        // (a bound for falls: r_top may be rounded up by more than t)
+        const float want = fmaxf(t, fminf(r_top - 40.0f - r_ref, kNew));
         const bool move = first || !(want >= kLow && want <= kHigh);
         // the previous PV has read P and written O^T
         if (n > 0 && !wait(pv_done, (uint32_t)(n - 1) & 1u)) { ok = false; break; }
         if (uint32_t moved = __ballot_sync(0xffffffffu, move)) {
-          const float by = move ? want - kNew : 0.0f;
-          const float f = fast_exp2(-by);
-          r_ref += by;
+          // O^T moves with the reference as it is held: next to one of 2^24 and
+          // more a step is wider than the window, and the difference to `by` is
+          // within the rounding of such scores
+          const float by = move ? want - kNew : 0.0f, r_new = r_ref + by;
+          const float f = fast_exp2(r_ref - r_new);
+          r_ref = r_new;
           if (!first) tc_fence_after();
 #pragma unroll
           for (int c = 0; c < HW; c += 8) {

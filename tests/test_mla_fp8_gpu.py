@@ -455,6 +455,21 @@ def test_decode_nan_tile_of_a_cut_sequence(gpu_ctx, B, tiles):
     assert torch.equal(out[1:], clean[1:]) and clean.isfinite().all()
 
 
+@pytest.mark.parametrize("H", [16, 64])
+@pytest.mark.parametrize("e", [26, 60, 90, 105])
+def test_decode_queries_of_any_finite_size(gpu_ctx, H, e):
+    """Queries near the end of the type's range: all weight on the best token, as in 64 bits, over several tiles."""
+    import torch
+
+    lens = [1000] * 45 + [64, 1]  # several tiles a run
+    q_lat, q_rope, cache, scales, table, scale = decode_inputs(lens, H, BIG, seed=70)
+    q_lat *= 2.0 ** e
+    q_rope *= 2.0 ** e
+    out = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, lens, scale)
+    gpu_ctx.sync()
+    check_decode(out, q_lat, q_rope, cache, scales, table, lens, scale)
+
+
 def test_decode_length_beyond_32_bit_positions_is_reported(gpu_ctx):
     """A table of 2^24 + 1 pages would hold it; positions past 2^30 are refused instead of wrapping."""
     import torch
