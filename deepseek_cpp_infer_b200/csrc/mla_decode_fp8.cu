@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           // the latents' scale; a rope part over 64 times larger sets it
           // instead (it is divided by the same factor, in bf16, exactly)
           const float top = redux_max(fmaxf(al, ar * 0.015625f));
-          const int e = min(100, max(-100, top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 7 : 0));
+          const int e = min(120, max(-100, top > 0.0f ? (int)(__float_as_uint(top) >> 23) - 127 - 7 : 0));
           const float inv = exp2i(-e);
           const uint64_t inv2 = pair(inv, inv);
           uint32_t hi[CPL / 4], lo[CPL / 4];

@@ -456,7 +456,7 @@ def test_decode_nan_tile_of_a_cut_sequence(gpu_ctx, B, tiles):
 
 
 @pytest.mark.parametrize("H", [16, 64])
-@pytest.mark.parametrize("e", [26, 60, 90, 105])
+@pytest.mark.parametrize("e", [26, 60, 90, 105, 107, 112, 119])
 def test_decode_queries_of_any_finite_size(gpu_ctx, H, e):
     """Queries near the end of the type's range: all weight on the best token, as in 64 bits, over several tiles."""
     import torch
