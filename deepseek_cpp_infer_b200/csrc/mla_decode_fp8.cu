@@ -715,8 +715,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         warp_arrive(&wg_bar[wg]);
         if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
         ++meet;
-        float t = fmaxf(fmaxf(red_n[hl], red_n[HW + hl]), fmaxf(red_n[2 * HW + hl], red_n[3 * HW + hl]));
-        if (t == -INFINITY) t = 0.0f;
+        const float t = fmaxf(fmaxf(red_n[hl], red_n[HW + hl]), fmaxf(red_n[2 * HW + hl], red_n[3 * HW + hl]));
         r_top = first ? t + r_ref : fmaxf(r_top, t + r_ref);
         // (a bound for falls: r_top may be rounded up by more than t)
         const float want = fmaxf(t, fminf(r_top - 40.0f - r_ref, kNew));
@@ -727,8 +726,10 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           // O^T moves with the reference as it is held: next to one of 2^24 and
           // more a step is wider than the window, and the difference to `by` is
           // within the rounding of such scores
-          const float by = move ? want - kNew : 0.0f, r_new = r_ref + by;
-          const float f = fast_exp2(r_ref - r_new);
+          // (-inf: no score yet that weighs anything, so O^T and the sums are zero,
+          // and stay it at a fall of any height)
+          const float by = move && want != -INFINITY ? want - kNew : 0.0f, r_new = r_ref + by;
+          const float f = fast_exp2(fminf(r_ref - r_new, 126.0f));
           r_ref = r_new;
           if (!first) tc_fence_after();
 #pragma unroll
@@ -849,7 +850,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
       }
       if (lane < HW) {
         mt[lane] = 1.0f / l;
-        if (!whole && quarter == 0) ws_ml[slot * HB + wg * HW + lane] = make_float2(r_ref, l);
+        if (!whole && quarter == 0) ws_ml[slot * HB + wg * HW + lane] = make_float2(l == 0.0f ? -3e38f : r_ref, l);
       }
       __syncwarp();
       if (!wait(pv_done, (uint32_t)n & 1u)) { ok = false; break; }

@@ -470,6 +470,30 @@ def test_decode_queries_of_any_finite_size(gpu_ctx, H, e):
     check_decode(out, q_lat, q_rope, cache, scales, table, lens, scale)
 
 
+@pytest.mark.parametrize("H", [16, 64])
+@pytest.mark.parametrize("n,none", [(1000, [0]), (1000, [0, 1, 2]), (1000, [3]), (1000, [7]), (260, [0, 1]), (19000, [0, 100])])
+def test_decode_tiles_of_infinitely_low_scores(gpu_ctx, H, n, none):
+    """Tiles whose scores are all -inf (infinite rope keys) weigh nothing and leave no mark on the others, whose scores
+    lie 200 below zero; in a run with others, in runs of their own, and in a whole sequence (NaN, as 0 / 0)."""
+    import torch
+
+    lens = [n, 300, 256] + [0] * 300  # (few runs a sequence, and runs with several sequences)
+    for B in (3, 303):
+        q_lat, q_rope, cache, scales, table, scale = decode_inputs(lens[:B], H, BIG, seed=60)
+        q_rope.zero_()
+        q_rope[..., 0] = 1.0
+        kr = torch.zeros(cache.shape[0], 64, 64, device="cuda")
+        kr[..., 0] = -200.0 / scale
+        for t in none:
+            kr[table[0, 2 * t:2 * t + 2].long(), :, 0] = -math.inf
+        kr[table[2, :4].long(), :, 0] = -math.inf
+        cache[..., 512:] = (kr / scales[..., None]).bfloat16().view(torch.uint8)
+        out = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, lens[:B], scale)
+        gpu_ctx.sync()
+        assert out[2].isnan().all()
+        check_decode(out[:2], q_lat[:2], q_rope[:2], cache, scales, table[:2], lens[:2], scale)
+
+
 def test_decode_length_beyond_32_bit_positions_is_reported(gpu_ctx):
     """A table of 2^24 + 1 pages would hold it; positions past 2^30 are refused instead of wrapping."""
     import torch
