@@ -13,11 +13,11 @@
 //
 // Precision.  An e4m3 value has 4 significant bits, a bf16 query 8: q / a (a
 // a power of two per head) is split into hi = e4m3(q / a) and lo = e4m3(q / a
-// - hi), exact down to 2^-18 of the head's largest value.  hi and lo are
+// - hi), to 2^-17 of the head's largest value.  hi and lo are
 // separate columns of one MMA (N = 2 heads), summed in fp32.  Probabilities
 // are split the same way (8 significant bits, like bf16) in units of a moving
-// reference per head that keeps every tile's largest within the digits' range
-// (see kLow), so that thousands of small probabilities behind one large one
+// reference per head that keeps what falls below the digits' steps small against
+// the sum (see kTileCost), so that thousands of small probabilities behind a large one
 // (an attention sink) keep their digits.  O^T accumulates in TMEM in fp32 and is
 // rescaled there when the reference moves.
 // The token's scale joins its probability: with u = s log2(e) + log2(sigma),
@@ -633,18 +633,27 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     };
 
     // Probabilities and sums are in units of 2^r, r a per-head reference (held
-    // by lane head % HW) that keeps each tile's largest probability between
-    // 1 and 430, whatever came before: a probability's digits are then off by
-    // at most 2^-8 of it, or 2^-10 (2^-14 with lo held 16-fold) where that is
-    // more.  (So with lo held plainly, equal probabilities of 2^-6 beside one of 1
-    // in every tile can all be off by 2^-4 of themselves; roundings that differ
-    // average out.)  When a tile's maximum leaves that window, the reference
-    // moves (to make it 16) and the head's columns of O^T are rescaled in TMEM;
-    // fp32 has the range for both directions (r never falls more than 2^40 below
-    // the largest: what lies further down is out of an fp32 sum's reach).
-    constexpr float kNew = 4.0f, kHigh = 8.75f, kLow = 0.0f;  // of the tile's maximum, in log2
+    // by lane head % HW).  Digits hold up to 448; a probability's are off by at
+    // most 2^-8 of it, or by 2^-10 (2^-14 with lo held 16-fold) where that is
+    // more.  A tile's 128 could thus lose 2^-3 (2^-7) together, if they all round
+    // the same way, while the sums take them whole.  The segment has to be worth
+    // it: of what its probabilities add up to at least (each warp's largest of
+    // every tile) a tile takes kTileCost, and `credit` is what is left.  A tile
+    // that it does not cover, or whose largest is above 2^kHigh, moves the
+    // reference, to make its largest 2^kNew, and the head's columns of O^T are
+    // rescaled in TMEM.  So this floor costs a segment at most 2^-3 / 32 = 2^-8
+    // (2^-7 / 8 = 2^-10) of the sum of its probabilities, no more than rounding
+    // each to bf16.  fp32 has the range for moves in both directions (r never falls
+    // more than 2^40 below the largest: what lies further down is out of an fp32
+    // sum's reach).  64 sequences of 1024 .. 8192, 128 heads: 132.5 us, a window
+    // [2^0, 2^8.75] for every tile's largest 127.5 (peaks could lose a tail of 11%
+    // of them), one that holds as much as the credit, [2^5, 2^8.75], 149; kTileCost
+    // 16 130.5; kNew 5 133.7, 7 135.3.
+    constexpr int DIG = S::DIG;
+    constexpr float kNew = DIG == 1 ? 6.0f : 5.0f, kHigh = 8.75f;  // log2
+    constexpr float kTileCost = DIG == 1 ? 32.0f : 8.0f;
     float ls[HW];  // softmax sums over this thread's tokens
-    float r_ref = 0.0f, r_top = 0.0f;
+    float r_ref = 0.0f, r_top = 0.0f, credit = 0.0f;
     if (lane < HW) mt[lane] = 0.0f;
     __syncwarp();
     int meet = 0;  // phase of wg_bar
@@ -715,11 +724,14 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
         warp_arrive(&wg_bar[wg]);
         if (!wait(&wg_bar[wg], (uint32_t)meet & 1u)) { ok = false; break; }
         ++meet;
-        const float t = fmaxf(fmaxf(red_n[hl], red_n[HW + hl]), fmaxf(red_n[2 * HW + hl], red_n[3 * HW + hl]));
+        const float t0 = red_n[hl], t1 = red_n[HW + hl], t2 = red_n[2 * HW + hl], t3 = red_n[3 * HW + hl];
+        const float t = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+        auto part = [](float v) { return fast_exp2(fminf(v, 100.0f)); };  // (finite: a move scales it down)
+        credit = (first ? 0.0f : credit) + ((part(t0) + part(t1)) + (part(t2) + part(t3)));
         r_top = first ? t + r_ref : fmaxf(r_top, t + r_ref);
         // (a bound for falls: r_top may be rounded up by more than t)
         const float want = fmaxf(t, fminf(r_top - 40.0f - r_ref, kNew));
-        const bool move = first || !(want >= kLow && want <= kHigh);
+        const bool move = first || !(want <= kHigh && credit >= kTileCost);
         // the previous PV has read P and written O^T
         if (n > 0 && !wait(pv_done, (uint32_t)(n - 1) & 1u)) { ok = false; break; }
         if (uint32_t moved = __ballot_sync(0xffffffffu, move)) {
@@ -731,6 +743,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           const float by = move && want != -INFINITY ? want - kNew : 0.0f, r_new = r_ref + by;
           const float f = fast_exp2(fminf(r_ref - r_new, 126.0f));
           r_ref = r_new;
+          credit *= f;
           if (!first) tc_fence_after();
 #pragma unroll
           for (int c = 0; c < HW; c += 8) {
@@ -748,15 +761,20 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
               fs[i] = __shfl_sync(0xffffffffu, f, c + i);
               ls[c + i] *= fs[i];
             }
+            constexpr int BLK = DIG == 1 && NL % 2 == 0 ? 2 : 1;  // blocks in flight (more spill)
 #pragma unroll 1
-            for (int g = 0; g < NL * S::DIG; ++g) {
+            for (int g = 0; g < NL * DIG; g += BLK) {
               const uint32_t at = t_lane + S::T_O + g * HB + wg * HW + c;
-              uint32_t o[8];
-              tmem_ld8(at, o);
+              uint32_t o[BLK][8];
+#pragma unroll
+              for (int k = 0; k < BLK; ++k) tmem_ld8(at + k * HB, o[k]);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fs[i]);
-              tmem_st8(at, o);
+              for (int k = 0; k < BLK; ++k) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[k][i] = __float_as_uint(__uint_as_float(o[k][i]) * fs[i]);
+                tmem_st8(at + k * HB, o[k]);
+              }
             }
           }
           if (!first) tmem_st_wait();
@@ -764,6 +782,7 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
           if (lane < HW) mt[lane] = -r_ref;
           __syncwarp();
         }
+        credit = fmaxf(credit - kTileCost, 0.0f);  // (less: beyond the bound for falls)
         // probabilities, their sums and digits
         uint32_t hi[HW / 4], lo[HW / 4];
 #pragma unroll

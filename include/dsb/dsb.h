@@ -384,9 +384,12 @@ DSB_API int dsb_kv_norm_rope_append_fp8(dsb_ctx* ctx, const float* kv_a, int64_t
  * row).  seq_lens is a DEVICE int32 [B]: the kernel splits the work itself, so
  * a captured call may be replayed with other lengths.  Cache rows past a
  * length are not used, whatever they hold.  A probability times its token's
- * scale is held to 2^-8 of its value, or 2^-14 (with R = 512 and more than 32
- * heads 2^-10) of the largest among its 128 tokens where that is more; sums are
- * in fp32.  Scales must be positive; a token whose scale is 2^-40 of its
+ * scale is held in two digits of 4 significant bits, to 2^-8 of its value; what
+ * small ones lose below the digits' steps is at most 2^-10 (with R = 512 and
+ * more than 32 heads 2^-8) of the sequence's sum of them.  A query is held to
+ * 2^-17 of its head's largest latent value, or 2^-23 of its largest rope value
+ * where that is more.  Sums are in fp32.
+ * Scales must be positive; a token whose scale is 2^-40 of its
  * sequence's largest or less may count as a zero row, one of scale 0 (a row
  * never written) counts as 2^-100.  Scratch comes
  * from the context (39 MB, allocated by the first call): calls of one context

@@ -292,6 +292,43 @@ def test_decode_equal_tail_beside_a_peak_in_every_tile(gpu_ctx, H):
     assert (err <= tol).all(), float((err / tol).max())
 
 
+@pytest.mark.parametrize("lead", [1.0, 2.0, 3.9, 15.0])
+@pytest.mark.parametrize("tail", [17.0, 0.9, 0.9 * 2.0 ** -2, 0.9 * 2.0 ** -5])
+@pytest.mark.parametrize("H", [16, 32, 64, 128])
+def test_decode_tail_below_the_digits_of_its_tile(gpu_ctx, H, tail, lead):
+    """A peak in every tile and 127 equal probabilities beside it, `tail` 2^-10 of the peak: around half a step of the
+    digits, where all can be lost together, and far below it; the first tile's peak is `lead` times the others'.  What
+    lies below the digits' steps costs a sequence at most 2^-8 of its probabilities (2^-10 up to 32 heads): at most
+    that much of a tile's mean latent."""
+
+    import torch
+
+    B, n, R = torch.cuda.get_device_properties(0).multi_processor_count, 1024, 512
+    lens = [n] * B
+    q_lat, q_rope, cache, scales, table, scale = decode_inputs(lens, H, BIG, seed=9)
+    q_lat.zero_()
+    q_rope.zero_()
+    q_rope[..., 0] = 1.0
+    unit = torch.full((n,), tail * 2.0 ** -10, dtype=torch.float64)
+    unit[5::128] = 1.0
+    unit[5] = lead
+    kr = torch.zeros(cache.shape[0], 64, 64, device="cuda")
+    kr[table.long(), :, 0] = (unit.log() / scale).float().cuda().view(1, -1, 64).expand(B, -1, -1)
+    codes, sc = ref.quantise(torch.randn(cache.shape[0], 64, R, device="cuda", dtype=torch.float64) * 0.1 + 1.0)
+    sc.fill_(2.0 ** -8)
+    cache[..., :R], scales[:] = codes, sc
+    cache[..., R:] = (kr / sc[..., None]).bfloat16().view(torch.uint8)
+    out = run_decode(gpu_ctx, q_lat, q_rope, cache, scales, table, lens, scale)
+    gpu_ctx.sync()
+    want, mag, _ = ref.decode64(q_lat, q_rope, cache, scales, table, lens, scale)
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * mag + 1e-30
+    for b in range(B):
+        lat, _ = ref.rows64(cache, scales, table, b, n, R)
+        tol[b] += 2.0 ** (-8 if H > 32 else -10) * lat.abs().view(-1, 128, R).mean(1).amax(0)
+    err = (out.double() - want).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
 def test_decode_scales_far_apart(gpu_ctx):
     """Token scales over 20 octaves and queries over 8: the largest tokens' latents dominate the output."""
     import torch
