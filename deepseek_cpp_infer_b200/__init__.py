@@ -478,21 +478,33 @@ class Context:
             block_table.data_ptr(), max_blocks, seq_lens.data_ptr(), B, H, R, P, softmax_scale, out.data_ptr()))
 
     def mla_cache_read_fp8(self, cache, scales, block_table, cu_seqlens, latent, k_rope):
-        """dsb_mla_cache_read_fp8: cached tokens as bf16 rows of latent [T, R] and k_rope [T, P]; cu_seqlens [B + 1]."""
-        T, R = latent.shape
-        P = k_rope.shape[1]
+        """dsb_mla_cache_read_fp8: cached tokens as bf16 rows of latent [T, R] and k_rope [T, P] (either may be None);
+        cu_seqlens [B + 1]."""
+        row = cache.shape[2]
+        if latent is not None:
+            T, R = latent.shape
+            P = (row - R) // 2 if k_rope is None else k_rope.shape[1]
+        elif k_rope is not None:
+            T, P = k_rope.shape
+            R = row - 2 * P
+        else:
+            raise ValueError("latent or k_rope wanted")
         blocks, (rows, max_blocks), B = cache.shape[0], block_table.shape, cu_seqlens.numel() - 1
         _need(self.device,
               ("cache", cache, "uint8", (blocks, 64, R + 2 * P), 0), ("scales", scales, "float32", (blocks, 64), 0),
               ("block_table", block_table, "int32", (rows, max_blocks), 0),
-              ("cu_seqlens", cu_seqlens, "int32", (B + 1,), 0), ("latent", latent, "bfloat16", (T, R), 1),
-              ("k_rope", k_rope, "bfloat16", (T, P), 1))
+              ("cu_seqlens", cu_seqlens, "int32", (B + 1,), 0))
+        if latent is not None:
+            _need(self.device, ("latent", latent, "bfloat16", (T, R), 1))
+        if k_rope is not None:
+            _need(self.device, ("k_rope", k_rope, "bfloat16", (T, P), 1))
         if rows < B:
             raise ValueError(f"block_table: {rows} rows for {B} sequences")
+        lat, ld_lat = (None, R) if latent is None else (latent.data_ptr(), latent.stride(0))
+        rope, ld_rope = (None, P) if k_rope is None else (k_rope.data_ptr(), k_rope.stride(0))
         self._check(self._l.dsb_mla_cache_read_fp8(
             self.h, cache.data_ptr(), scales.data_ptr(), blocks, block_table.data_ptr(), max_blocks,
-            cu_seqlens.data_ptr(), B, T, R, P, latent.data_ptr(), latent.stride(0), k_rope.data_ptr(),
-            k_rope.stride(0)))
+            cu_seqlens.data_ptr(), B, T, R, P, lat, ld_lat, rope, ld_rope))
 
     def mla_prefill(self, q_nope, q_rope, k_nope, k_rope, v, cu_q, cu_k, max_q, softmax_scale, out, causal=True,
                     lse=None):

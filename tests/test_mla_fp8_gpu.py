@@ -568,6 +568,25 @@ def test_read_back_is_exact(gpu_ctx, lens, shape):
     assert (lat[T:] == 7.0).all() and (rope[T:] == 7.0).all() and (lat[:, R:] == 7.0).all() and (rope[:, P:] == 7.0).all()
 
 
+@pytest.mark.parametrize("shape", [BIG, SMALL])
+def test_read_of_one_part(gpu_ctx, shape):
+    """Only the latents, or only the rope keys."""
+    import torch
+
+    R, P, _ = shape
+    lens = [70, 1, 200]
+    table, n_blocks = ref.make_table(lens, seed=5)
+    cache, scales = ref.make_cache(n_blocks, R, P, seed=6)
+    cu = torch.tensor([0, 70, 71, 271], dtype=torch.int32, device="cuda")
+    lat, rope = torch.zeros(271, R, dtype=torch.bfloat16, device="cuda"), torch.zeros(271, P, dtype=torch.bfloat16, device="cuda")
+    gpu_ctx.mla_cache_read_fp8(cache, scales, table, cu, lat, None)
+    gpu_ctx.mla_cache_read_fp8(cache, scales, table, cu, None, rope)
+    gpu_ctx.sync()
+    want = [ref.rows64(cache, scales, table, b, n, R) for b, n in enumerate(lens)]
+    assert torch.equal(lat.double(), torch.cat([w[0] for w in want]))
+    assert torch.equal(rope.double(), torch.cat([w[1] for w in want]))
+
+
 def test_read_every_code(gpu_ctx):
     """All 256 e4m3 codes (NaN among them) and scales from 2^-64 to 2^64."""
     import torch

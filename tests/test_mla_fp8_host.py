@@ -123,3 +123,29 @@ def test_append_refuses_rows_narrower_than_a_token(name, cut, B):
     with pytest.raises(ValueError, match=name):
         ctx.kv_norm_rope_append_fp8(**{**a, name: a[name][:, cut]})
     assert len(ctx._l.calls) == 1
+
+
+def read_args(T, R=128, P=32):
+    import torch
+
+    return dict(cache=torch.zeros(4, 64, R + 2 * P, dtype=torch.uint8), scales=torch.ones(4, 64),
+                block_table=torch.zeros(1, 1, dtype=torch.int32), cu_seqlens=torch.tensor([0, T], dtype=torch.int32),
+                latent=torch.zeros(T, R).bfloat16(), k_rope=torch.zeros(T, P).bfloat16())
+
+
+def test_read_of_one_part():
+    """Either output may be left out, as at the C entry point; not both."""
+    import torch
+
+    ctx, a = binding(), read_args(5)
+    ctx.mla_cache_read_fp8(**a)
+    ctx.mla_cache_read_fp8(**{**a, "latent": None})
+    ctx.mla_cache_read_fp8(**{**a, "k_rope": None})
+    both, rope, lat = (c[1] for c in ctx._l.calls)
+    assert both[8:11] == rope[8:11] == lat[8:11] == (5, 128, 32)  # T, R, P
+    assert rope[11] is None and rope[13:] == both[13:]
+    assert lat[13] is None and lat[11:13] == both[11:13]
+    with pytest.raises(ValueError):
+        ctx.mla_cache_read_fp8(**{**a, "latent": None, "k_rope": None})
+    with pytest.raises(ValueError):  # 192 bytes a row: R + 2P
+        ctx.mla_cache_read_fp8(**{**a, "k_rope": None, "latent": torch.zeros(5, 129).bfloat16()})
