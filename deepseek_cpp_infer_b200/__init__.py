@@ -299,6 +299,11 @@ def _need(device: int, *wanted):
             step *= shape[i]
 
 
+def _pitch(t, dim: int, dense: int) -> int:
+    """The stride of a dimension; `dense` where it has one element or none, whose stride may be anything."""
+    return t.stride(dim) if t.shape[dim] > 1 else dense
+
+
 class Context:
     """One dsb_ctx: a device, a stream, a workspace and counters."""
 
@@ -456,7 +461,8 @@ class Context:
         if seq_ids is not None:
             _need(self.device, ("seq_ids", seq_ids, "int32", (B,), 0))
         self._check(self._l.dsb_kv_norm_rope_append_fp8(
-            self.h, kv_a.data_ptr(), kv_a.stride(0), w_norm.data_ptr(), q.data_ptr(), q.stride(0),
+            self.h, kv_a.data_ptr(), _pitch(kv_a, 0, R + P), w_norm.data_ptr(), q.data_ptr(),
+            _pitch(q, 0, H * (nope + P)),
             positions.data_ptr(), _ptr(seq_ids), block_table.data_ptr(), rows, max_blocks, B, H, nope, R, P, eps, theta,
             cache.data_ptr(), scales.data_ptr(), blocks, q_rope.data_ptr()))
 
@@ -500,8 +506,8 @@ class Context:
             _need(self.device, ("k_rope", k_rope, "bfloat16", (T, P), 1))
         if rows < B:
             raise ValueError(f"block_table: {rows} rows for {B} sequences")
-        lat, ld_lat = (None, R) if latent is None else (latent.data_ptr(), latent.stride(0))
-        rope, ld_rope = (None, P) if k_rope is None else (k_rope.data_ptr(), k_rope.stride(0))
+        lat, ld_lat = (None, R) if latent is None else (latent.data_ptr(), _pitch(latent, 0, R))
+        rope, ld_rope = (None, P) if k_rope is None else (k_rope.data_ptr(), _pitch(k_rope, 0, P))
         self._check(self._l.dsb_mla_cache_read_fp8(
             self.h, cache.data_ptr(), scales.data_ptr(), blocks, block_table.data_ptr(), max_blocks,
             cu_seqlens.data_ptr(), B, T, R, P, lat, ld_lat, rope, ld_rope))
@@ -519,15 +525,20 @@ class Context:
               ("cu_q", cu_q, "int32", (n,), 0), ("cu_k", cu_k, "int32", (n,), 0))
         if lse is not None:
             _need(self.device, ("lse", lse, "float32", (Tq, H), 0))
+        def pitches(t):
+            hd = _pitch(t, 1, t.shape[2])
+            return _pitch(t, 0, H * hd), hd
+
+        (ld_qn, hd_qn), (ld_qr, hd_qr), (ld_kn, hd_kn), (ld_v, hd_v) = map(pitches, (q_nope, q_rope, k_nope, v))
         a = MlaPrefillArgs(
-            q_nope=q_nope.data_ptr(), ld_q_nope=q_nope.stride(0), hd_q_nope=q_nope.stride(1),
-            q_rope=q_rope.data_ptr(), ld_q_rope=q_rope.stride(0), hd_q_rope=q_rope.stride(1),
-            k_nope=k_nope.data_ptr(), ld_k_nope=k_nope.stride(0), hd_k_nope=k_nope.stride(1),
-            k_rope=k_rope.data_ptr(), ld_k_rope=k_rope.stride(0),
-            v=v.data_ptr(), ld_v=v.stride(0), hd_v=v.stride(1),
+            q_nope=q_nope.data_ptr(), ld_q_nope=ld_qn, hd_q_nope=hd_qn,
+            q_rope=q_rope.data_ptr(), ld_q_rope=ld_qr, hd_q_rope=hd_qr,
+            k_nope=k_nope.data_ptr(), ld_k_nope=ld_kn, hd_k_nope=hd_kn,
+            k_rope=k_rope.data_ptr(), ld_k_rope=_pitch(k_rope, 0, P),
+            v=v.data_ptr(), ld_v=ld_v, hd_v=hd_v,
             cu_q=cu_q.data_ptr(), cu_k=cu_k.data_ptr(), B=n - 1, Tq=Tq, Tk=Tk, max_q=int(max_q), H=H,
             nope=nope, P=P, vd=vd, causal=int(causal), softmax_scale=softmax_scale,
-            out=out.data_ptr(), ld_out=out.stride(0), lse=_ptr(lse),
+            out=out.data_ptr(), ld_out=_pitch(out, 0, H * vd), lse=_ptr(lse),
         )
         self._check(self._l.dsb_mla_prefill(self.h, ctypes.byref(a)))
 

@@ -149,3 +149,59 @@ def test_read_of_one_part():
         ctx.mla_cache_read_fp8(**{**a, "latent": None, "k_rope": None})
     with pytest.raises(ValueError):  # 192 bytes a row: R + 2P
         ctx.mla_cache_read_fp8(**{**a, "k_rope": None, "latent": torch.zeros(5, 129).bfloat16()})
+
+
+def odd_row(t, stride=1):
+    """The same single row with a first stride that says nothing (as after a transposition)."""
+    import torch
+
+    assert t.shape[0] == 1
+    return torch.as_strided(t, t.shape, (stride, *t.stride()[1:]))
+
+
+@pytest.mark.parametrize("stride", [1, 3, 8])
+def test_one_row_of_any_stride(stride):
+    """The stride of a dimension of one element is arbitrary: the library gets the row's own width."""
+    import torch
+
+    ctx, a = binding(), append_args(B=1)
+    ctx.kv_norm_rope_append_fp8(**a)
+    ctx.kv_norm_rope_append_fp8(**{**a, "kv_a": odd_row(a["kv_a"], stride), "q": odd_row(a["q"], stride)})
+    ctx.kv_norm_rope_append_fp8(**{**a, "kv_a": torch.zeros(1, 161)[:, :160], "q": torch.zeros(1, 193).bfloat16()})
+    first, second, third = (c[1] for c in ctx._l.calls)
+    assert first == second and first[2] == third[2] == 160 and first[5] == third[5] == 192
+    ctx, a = binding(), read_args(1)
+    ctx.mla_cache_read_fp8(**a)
+    ctx.mla_cache_read_fp8(**{**a, "latent": odd_row(a["latent"], stride), "k_rope": odd_row(a["k_rope"], stride)})
+    assert ctx._l.calls[0][1] == ctx._l.calls[1][1]
+
+
+def test_one_prompt_row_or_head_of_any_stride():
+    import torch
+
+    def x(*shape):
+        return torch.zeros(*shape).bfloat16()
+
+    cu, seen = torch.tensor([0, 1], dtype=torch.int32), []
+    for T, H in ((1, 4), (1, 1), (5, 1)):
+        kv = x(T, H, 128)
+        a = dict(q_nope=x(T, H, 64), q_rope=x(T, H, 32), k_nope=kv[..., :64], k_rope=x(T, 32), v=kv[..., 64:],
+                 cu_q=cu, cu_k=cu, max_q=T, softmax_scale=0.1, out=x(T, H, 64))
+        for odd in (False, True):
+            b = dict(a)
+            if odd:  # the dimensions of one element get a stride of 1
+                for k, t in a.items():
+                    if isinstance(t, torch.Tensor) and t.dtype == torch.bfloat16:
+                        b[k] = torch.as_strided(t, t.shape, [1 if n == 1 else s for n, s in zip(t.shape, t.stride())],
+                                                t.storage_offset())
+            ctx = binding()
+            ctx.mla_prefill(**b)
+            p = ctx._l.calls[0][1][1]._obj
+            for name, dim, heads in (("q_nope", 64, H), ("q_rope", 32, H), ("k_nope", 64, H), ("k_rope", 32, 1), ("v", 64, H)):
+                ld, hd = getattr(p, "ld_" + name), getattr(p, "hd_" + name) if name != "k_rope" else dim
+                assert ld % 8 == 0 and hd % 8 == 0 and hd >= dim and ld >= (heads - 1) * hd + dim, (T, H, odd, name)
+                if heads > 1:
+                    assert hd == a[name].stride(1)
+                if T > 1:
+                    assert ld == a[name].stride(0)
+            assert p.ld_out == H * 64

@@ -236,6 +236,21 @@ def test_output_pitch_and_no_lse(gpu_ctx):
     assert (wide[:, 384:] == 7.0).all()
 
 
+@pytest.mark.parametrize("T,H", [(1, 4), (1, 1), (70, 1)])
+def test_one_row_or_head_of_any_stride(gpu_ctx, T, H):
+    """Dimensions of one element whose strides (1) are no pitches."""
+    import torch
+
+    x = inputs([T], [T], H, BIG, seed=16)
+    out, lse = run(gpu_ctx, x, [T], [T])
+    odd = [torch.as_strided(t, t.shape, [1 if n == 1 else s for n, s in zip(t.shape, t.stride())], t.storage_offset())
+           for t in x[:5]]
+    out2, lse2 = run(gpu_ctx, (*odd, x[5]), [T], [T])
+    gpu_ctx.sync()
+    check(out2, lse2, x, [T], [T])
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
 def test_max_q_too_small_is_reported(gpu_ctx):
     lq = [100, 300]
     x = inputs(lq, lq, 2, BIG, seed=10)
