@@ -36,16 +36,18 @@
 // and, as soon as its block of O^T is done, is free again.
 //
 // What bounds it.  16 heads (12 slabs): HBM; 64 sequences of 1024 .. 8192
-// tokens take 39 us, 5.0 TB/s with all overheads, and a tile's 3100 cycles in
+// tokens take 41 us, 4.8 TB/s with all overheads, and a tile's 3100 cycles in
 // mid-run are the copy rate.  64 heads (72 KB of query digits leave 8 slabs):
 // the chain of a tile, about 5000 cycles against 2840 of MMAs: PV's first block
 // frees a slab, the next tile's last slab is loaded into it (1300 - 1900), QK,
-// softmax (1900), PV.  128 heads, the same sequences: 120 us, 700 TFLOP/s; 32 of
-// 4112 tokens 64 us; 3 of 60000 .. 131072 tokens 107 us.  At a sequence's end a
-// run takes another 14000 cycles for its output and the next query's digits.
-// One short sequence takes 11.1 us with the merge, two launches and a tile's
+// softmax (1900), PV.  128 heads, the same sequences: 132 us, 640 TFLOP/s; 32 of
+// 4112 tokens 67 us; 3 of 60000 .. 131072 tokens (344,000 in all) 125 us.  At a
+// sequence's end a run takes another 14000 cycles for its output and the next
+// query's digits; the runs have equal tiles whatever ends they hold.
+// One short sequence takes 11.2 us with the merge, two launches and a tile's
 // chain.
-// What did not help: O^T accumulated in registers per tile, one warp for QK
+// What did not help (all figures of this paragraph: 128 heads, when the kernel
+// took 120 - 130 us): O^T accumulated in registers per tile, one warp for QK
 // and PV, four softmax warpgroups, 48 heads per CTA (9 slabs, 138 us), a
 // reference that lags one tile behind (168 us), partials of four heads a
 // float4 (134 us).  At 64 heads the softmax warps use all 168 registers that
@@ -956,6 +958,10 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
 // so many CTAs cost more (64 x 64 75.1 against 77.4 us, 74 x 128 whole sequences
 // 15.5 against 24.0).  Without the merge those four take 12.5, 37.7, 69.8, 13.4.
 constexpr int kCombineWarps = 8;
+// The border is that of 16 heads (513 .. 768 tokens: 24 sequences 12.5 us by a
+// CTA a head, 13.5 by a warp a part; 32 14.7 and 14.9; 48 16.8 and 15.9).  With
+// more heads it lies lower: 64 heads, 8 sequences 17.6 and 18.4, 16 19.5 and
+// 18.9; 128 heads, 4 17.7 and 18.4, 8 19.6 and 18.7, 24 33.7 and 27.9.
 constexpr int kFewFrom = 32;         // sequences
 constexpr int kSplitRows = 2048;     // sequences x heads up to which V = 1
 
@@ -1157,7 +1163,9 @@ extern "C" int dsb_mla_decode_fp8(dsb_ctx* ctx, const void* q_lat, const void* q
     return f(ctx, q_lat, q_rope, cache, scales, n_blocks, block_table, max_blocks, seq_lens, B, H, softmax_scale,
              out_lat);
   };
-  // the fewest columns that hold the heads: a tile's MMA time grows with them
+  // the fewest columns of 16, 32 and 64 that hold the heads, or groups of 64: a
+  // tile's MMA time grows with them (64 sequences, 16 heads 41 us, 32 50, 64 80,
+  // 96 and 128 128 - 132; two groups of 48 took 138 when two of 64 took 130)
   if (R == 512) return H <= 16 ? run(launch<512, 64, 16>) : H <= 32 ? run(launch<512, 64, 32>) : run(launch<512, 64, 64>);
   return H <= 16 ? run(launch<128, 32, 16>) : H <= 32 ? run(launch<128, 32, 32>) : run(launch<128, 32, 64>);
 }

@@ -23,12 +23,19 @@
 // first within groups of heads whose keys and values stay in L2; an item's
 // prologue overlaps the last one's epilogue.
 //
-// Bound by the tensor core and, before it, by power: at 128 heads one prompt
-// of 4096 rows (causal) takes 708 us and 1024 rows behind 3000 keys 283 us,
-// 970 - 1050 TFLOP/s at 1.6 - 1.75 GHz under the 1000 W limit (cuBLAS sustains
-// 1386 there); 32 prompts of 512 rows at 16 heads 85 us, 1.8 times the
-// time of their bytes: an item is only 1 to 4 steps long, so that its Q load,
-// first softmax and output show.  What did not help: an MMA warp for each tile
+// What bounds it.  With equal items (2048 rows, 128 heads, no causal mask) 311 us,
+// 1104 TFLOP/s: a step's softmax and hand-overs, which only the other tile's MMAs
+// hide (2048 causal rows: the tensor pipe at 38%).  Causal prompts lose more
+// to the items' fixed stride: they differ in length, and the same CTAs get the
+// long ones of every round, so that with an item counted as its steps and one
+// the most loaded SM has 324 of a mean 249 at 4096 rows x 128 heads (710 - 810 us
+// by GPU and power, 860 - 970 TFLOP/s), 124 of 104 at 1024 rows behind 3000 keys
+// (280 - 330 us), 48 of 31 at 4096 rows x 16 heads (105 us) and 31 of 16 at prompts
+// of 2048, 1500, 600 and 100 rows; handed to whichever CTA is free they would
+// have 253, 118, 33 and 19.  Long calls at 128 heads also run at 1.6 - 1.75 GHz
+// under the 1000 W limit.  32 prompts of 512 rows at 16 heads take 83 - 91 us, 2
+// times the time of their bytes: an item is only 1 to 4 steps long, so that its Q
+// load, first softmax and output show.  What did not help: an MMA warp for each tile
 // (15% slower: the tiles fall into step), two softmax warpgroups a tile, P
 // handed over in halves, part of the exponentials as polynomials, the next
 // item's first scores ahead of this item's output.

@@ -345,7 +345,7 @@ DSB_API int dsb_kv_norm_rope_append(dsb_ctx* ctx, const float* kv_a, const float
  * token's own power of two (a page-wide one would have to be requantised as
  * tokens arrive; e4m3 carries an exponent, so a power of two costs range and
  * no precision), and it covers the whole row: the rope part is the bf16 rope
- * key divided by it, which is exact.  Every cached value is therefore exact
+ * key divided by it, which is exact where the quotient is within bf16's range.  Every cached value is therefore exact
  * in bf16.  The reference caches fp32 keys and values (MLACache,
  * src/models/deepseek/mla.cpp:16-39) and has no 8-bit cache.
  *
@@ -424,7 +424,10 @@ DSB_API int dsb_mla_cache_read_fp8(dsb_ctx* ctx, const void* cache, const float*
  * cu_q[b] .. cu_q[b+1] and key rows cu_k[b] .. cu_k[b+1] (device int32 [B + 1],
  * ascending from 0, at most Tq and Tk); with `causal`, its i-th query sees
  * its keys j <= i + len_k - len_q (the last query sees every key).  A query
- * that sees none gets a zero row and lse = -inf.  Query rows at or past
+ * that sees none gets a zero row and lse = -inf.  Scores, their statistics and
+ * all sums are in fp32; a probability is rounded to bf16 (2^-8 of it) before its
+ * product with v, the sums and lse take it unrounded.  Keys and values that a
+ * query does not see do not change its row, whatever they hold.  Query rows at or past
  * cu_q[B] are left as they were.  max_q bounds any sequence's query rows: it
  * sizes the grid, and rows beyond it set the status word (dsb_sync returns
  * DSB_EINVAL) and are left as they were.
