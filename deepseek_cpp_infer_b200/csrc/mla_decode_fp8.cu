@@ -650,7 +650,9 @@ __global__ void __launch_bounds__(Shape<R, P, HB>::THREADS, 1)
     // sum's reach).  64 sequences of 1024 .. 8192, 128 heads: 132.5 us, a window
     // [2^0, 2^8.75] for every tile's largest 127.5 (peaks could lose a tail of 11%
     // of them), one that holds as much as the credit, [2^5, 2^8.75], 149; kTileCost
-    // 16 130.5; kNew 5 133.7, 7 135.3.
+    // 16 130.5; kNew 5 133.7, 7 135.3.  (Scores there have a deviation of 1.7.  Of
+    // 3.5 and 7: 143 - 146 and 149 - 151 us, by the first window 146 - 148 and 153
+    // - 155: its moves do not count what later tiles are worth.  Equal ones: 124.)
     constexpr int DIG = S::DIG;
     constexpr float kNew = DIG == 1 ? 6.0f : 5.0f, kHigh = 8.75f;  // log2
     constexpr float kTileCost = DIG == 1 ? 32.0f : 8.0f;
